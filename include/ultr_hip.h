@@ -70,6 +70,7 @@ extern "C" {
 #define ULTR_MAX_LIST 64     /* max rank_list_size for the loss / feed kernels   */
 #define ULTR_MAX_SORT 2048   /* max list length for the metric sort              */
 #define ULTR_MAX_WIDTH 1024  /* max hidden width                                 */
+#define ULTR_MAX_NORM_WIDTH 65536 /* max row width of ultr_layer_norm_*        */
 #define ULTR_FEED_INFO_INTS 1088 /* int32 words of the feed kernels' `info` array  */
 
 /* activation_func (base_ranking_model.py:59-65) */
@@ -95,8 +96,9 @@ enum { ULTR_OPT_ADAGRAD = 0, ULTR_OPT_SGD = 1 };
  * operands (activations and gradients rounded on the fly, weights from packed bf16 copies that the update launch keeps
  * current) and accumulate in fp32; LayerNorm, activations, losses, the output layer, the split-K reduction and the
  * optimiser stay fp32, what the step writes to memory stays fp32, and the parameters are fp32 master copies.
- * Stated error bound: DESIGN.md section 3. */
-enum { ULTR_DTYPE_F32 = 0, ULTR_DTYPE_BF16 = 1 };
+ * Stated error bound: DESIGN.md section 3.
+ * F16 is a storage type of the stand-alone operators (layer norm, tensor lists) only; a scorer refuses it. */
+enum { ULTR_DTYPE_F32 = 0, ULTR_DTYPE_BF16 = 1, ULTR_DTYPE_F16 = 2 };
 /* metric bits for ultr_metrics */
 enum { ULTR_METRIC_MRR = 1, ULTR_METRIC_NDCG = 2, ULTR_METRIC_ERR = 4 };
 
@@ -247,6 +249,31 @@ int ultr_online_sample_click(float tau, const double* rank_uniforms, const int* 
                              const double* uniforms, unsigned long long seed, unsigned int step,
                              const unsigned int* step_ctr, unsigned int slot_base, int check_validation, int max_rounds,
                              int* out_docids, float* out_clicks, int* out_perm, void* stream);
+
+/* ---- layer normalisation as an operator (base_ranking_model.py:67-70 NORM_FUNC_DIC, DNN.py:78-81) --------
+ * Rows of a tensor of the caller's own, where the scorer below has LayerNorm fused into its GEMMs.  For row m < M over
+ * its N entries, with v the biased variance:
+ *   stats[m] = (mean, rstd = 1/sqrt(v + eps)) ;  y = (x - mean) * rstd * gamma + beta
+ * x, y: [M][N] of x_dtype (ULTR_DTYPE_F32 / BF16 / F16), rows ldx / ldy ELEMENTS apart (>= N; the entries of a row are
+ * contiguous), any alignment of the element type.  gamma, beta: [N] of w_dtype (ULTR_DTYPE_F32 or x_dtype), each may
+ * be NULL (1 and 0).  stats: [M][2] fp32, the layout of ultr_ln_row_stats, 8-byte aligned; may be NULL.
+ * Everything between load and store is fp32; the mean is formed before the variance.  y may be x itself (same pointer
+ * and stride); any other overlap of the two is refused.  M = 0 is a no-op.  A row holding a NaN or an infinity gives
+ * NaN in that row only.  1 <= N <= ULTR_MAX_NORM_WIDTH, eps > 0. */
+int ultr_layer_norm_forward(const void* x, long long ldx, const void* gamma, const void* beta, long long M, int N,
+                            float eps, int x_dtype, int w_dtype, void* y, long long ldy, float* stats, void* stream);
+
+/* Its gradient.  With xh = (x - mean) * rstd from the forward pass's stats and g = dy * gamma:
+ *   dx = rstd * (g - mean_N(g) - xh * mean_N(g * xh)) ;  d_gamma = sum_m dy * xh ;  d_beta = sum_m dy
+ * dy, dx as x above (lddy, lddx); d_gamma, d_beta: [N] of w_dtype, written, not added to (zeros when M = 0).
+ * dx, d_gamma and d_beta may each be NULL (not wanted), not all of them.  dx must not overlap x or dy.
+ * The sums over rows are fp32 in an order that depends on (M, N, types) only: equal calls give equal bits.
+ * ws: ultr_layer_norm_workspace_bytes(M, N) bytes, 16-byte aligned, contents irrelevant before and after the call; may
+ * be NULL when that is 0 or when neither d_gamma nor d_beta is wanted.  Two calls in flight need a workspace each. */
+long long ultr_layer_norm_workspace_bytes(long long M, int N);
+int ultr_layer_norm_backward(const void* dy, long long lddy, const void* x, long long ldx, const float* stats,
+                             const void* gamma, long long M, int N, int x_dtype, int w_dtype, void* dx, long long lddx,
+                             void* d_gamma, void* d_beta, void* ws, void* stream);
 
 /* ---- DNN scorer (DNN.py:48-96 via base_algorithm.py:104-134) ---------------------------- */
 /* Bytes of workspace ultr_dnn_forward/backward need for M rows (M = L*B). */
@@ -527,6 +554,59 @@ int ultr_clip_adagrad3(float* theta, float* acc, const float* grads, long long n
                        const float* denom_s, float scale_const_s, float l2_s, float clip_norm_s, float lr_s,
                        float* out_norm_s, const float* sumsq, int n_sumsq, long long n_covered,
                        const float* publish_src, float* publish_dst, int publish_n, void* stream);
+
+/* ---- global norm, clipping and the update over MANY tensors (tf.clip_by_global_norm + apply_gradients over the
+ * variable list, dla.py:237-255; ipw_rank.py:155-165) -----------------------------------------------------------------
+ * The calls above work on one flat fp32 buffer.  These take a list of separate tensors of any size and alignment:
+ * gradients in fp32, bf16 or fp16 and, for the update, fp32 parameters and accumulators, with an optional bf16 / fp16
+ * copy of each updated parameter.  The list is laid out once, by ultr_tensors_plan, into a device table that the
+ * caller owns; the later calls read the tensors' CURRENT values through it. */
+typedef struct UltrTensor {
+  const void* grad;   /* [n] of grad_dtype                                                              */
+  void* out;          /* [n] of grad_dtype: where ultr_clip_by_global_norm writes; may be grad or NULL  */
+  float* param;       /* [n] or NULL                                                                    */
+  float* accum;       /* [n] or NULL                                                                    */
+  void* copy;         /* [n] of copy_dtype, rewritten from param by the update; may be NULL             */
+  long long n;        /* elements; 0 is allowed (pointers are then ignored)                             */
+  int grad_dtype;     /* ULTR_DTYPE_*                                                                   */
+  int copy_dtype;     /* ULTR_DTYPE_* (ignored without copy)                                            */
+} UltrTensor;
+typedef struct UltrTensorPlan {
+  void* table;        /* device memory given to ultr_tensors_plan                                       */
+  long long n_chunks; /* the list cut into chunks, none of which spans two tensors                      */
+  int n_tensors;
+  int has;            /* bits of what EVERY non-empty tensor has: 1 out, 2 param, 4 accum               */
+} UltrTensorPlan;
+
+/* Device bytes the table of this list takes (> 0 even for an empty list); -1 on a bad list. */
+long long ultr_tensors_table_bytes(const UltrTensor* tensors_h, int n_tensors);
+/* Fills `table` (16-byte aligned, table_bytes at least the above) by kernels on `stream` -- no copy from host memory, so
+ * tensors_h may be dropped at once -- and *plan_h.  Calls that use the plan must be ordered behind this one.  The table
+ * holds the tensors' addresses: it is void once one of them is freed.  It also holds the partial sums of a call in
+ * flight: calls (or replays of captured graphs) with one plan must be ordered one after the other.
+ * Refused: memory the calls would write (out, param, accum, copy) that overlaps any other tensor of the list, other than
+ * out == grad of one tensor. */
+int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, void* table, long long table_bytes,
+                      UltrTensorPlan* plan_h, void* stream);
+
+/* out_norm[0] = sqrt(sum over all tensors of (scale * g)^2), scale = scale_const / denom[0] (denom NULL: scale_const),
+ * as ultr_clip_adagrad scales.  The products are fp32, their squares are summed in 64 bits in an order fixed by the
+ * plan, so the norm neither overflows nor vanishes before fp32 itself does; an empty list gives 0. */
+int ultr_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float* out_norm, void* stream);
+
+/* out = f * scale * grad for every tensor, f = clip_norm / max(norm, clip_norm) with the norm above (also written to
+ * out_norm if that is not NULL).  clip_norm <= 0: f = 1.  A norm that is not finite makes f NaN, and so every output
+ * NaN (tf.clip_by_global_norm).  Needs `out` in every tensor. */
+int ultr_clip_by_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float clip_norm,
+                             float* out_norm, void* stream);
+
+/* The update of ultr_clip_adagrad over the list: e = scale * g + l2 * theta, norm over all e (0 with clip_norm <= 0 and
+ * out_norm NULL: not formed), e *= f, Adagrad: acc += e^2, theta -= lr * e / sqrt(acc); SGD: theta -= lr * e; then
+ * copy = theta rounded to copy_dtype.  Gradients are left as they are.  Needs `param` in every tensor, and `accum` for
+ * Adagrad.  f as above: a norm that is not finite makes every updated value NaN when clip_norm > 0. */
+int ultr_clip_adagrad_tensors(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float l2,
+                              float clip_norm, float lr, int strategy, float* out_norm, void* stream);
+
 
 /* ultr_clip_adagrad3 for a scorer that trains through ultr_dnn_train_fused: the update launch also writes the updated
  * hidden-layer weight matrices, transposed, into the fused step's workspace (same desc, B, L), so the next

@@ -13,11 +13,12 @@ LIB_PATH = os.path.join(_HERE, 'csrc', 'libultr_hip.so')
 
 ULTR_MAX_LAYERS = 8
 ULTR_MAX_LIST = 64
+ULTR_MAX_NORM_WIDTH = 65536
 ULTR_FEED_INFO_INTS = 1088
 
 ACT = {'elu': 0, 'relu': 1, 'selu': 2, 'tanh': 3, 'sigmoid': 4}
 NORM_NONE, NORM_LAYER, NORM_BATCH, NORM_BATCH_EVAL = 0, 1, 2, 3
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 CLICK_PBM, CLICK_CASCADE, CLICK_ORACLE, CLICK_TABLE, CLICK_UBM = 0, 1, 2, 3, 4
 LOSS_SOFTMAX, LOSS_SIGMOID = 0, 1
 PROB_SOFTMAX, PROB_SIGMOID = 0, 1
@@ -47,6 +48,28 @@ class UltrDnnDesc(ctypes.Structure):
     ]
 
 
+class UltrTensor(ctypes.Structure):
+    _fields_ = [
+        ('grad', ctypes.c_void_p),
+        ('out', ctypes.c_void_p),
+        ('param', ctypes.c_void_p),
+        ('accum', ctypes.c_void_p),
+        ('copy', ctypes.c_void_p),
+        ('n', ctypes.c_longlong),
+        ('grad_dtype', ctypes.c_int),
+        ('copy_dtype', ctypes.c_int),
+    ]
+
+
+class UltrTensorPlan(ctypes.Structure):
+    _fields_ = [
+        ('table', ctypes.c_void_p),
+        ('n_chunks', ctypes.c_longlong),
+        ('n_tensors', ctypes.c_int),
+        ('has', ctypes.c_int),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _U = ctypes.c_uint
@@ -54,6 +77,8 @@ _LL = ctypes.c_longlong
 _ULL = ctypes.c_ulonglong
 _F = ctypes.c_float
 _DESC = ctypes.POINTER(UltrDnnDesc)
+_TENSOR = ctypes.POINTER(UltrTensor)
+_PLAN = ctypes.POINTER(UltrTensorPlan)
 
 # name -> (restype, argtypes); mirrors include/ultr_hip.h one to one
 SIGNATURES = {
@@ -66,6 +91,9 @@ SIGNATURES = {
     'ultr_profile_enable': (_I, [_I]),
     'ultr_profile_report': (_I, [ctypes.c_char_p, _I]),
     'ultr_ln_row_stats': (_I, [_P, _LL, _I, _I, _F, _P, _P]),
+    'ultr_layer_norm_forward': (_I, [_P, _LL, _P, _P, _LL, _I, _F, _I, _I, _P, _LL, _P, _P]),
+    'ultr_layer_norm_workspace_bytes': (_LL, [_LL, _I]),
+    'ultr_layer_norm_backward': (_I, [_P, _LL, _P, _LL, _P, _P, _LL, _I, _I, _I, _P, _LL, _P, _P, _P, _P]),
     'ultr_click_pbm': (_I, [_P, _LL, _I, _P, _I, _P, _I, _P, _ULL, _U, _P, _P]),
     'ultr_click_sample': (_I, [_I, _P, _LL, _I, _P, _I, _P, _I, _P, _ULL, _U, _P, _P]),
     'ultr_click_cascade': (_I, [_P, _LL, _I, _P, _I, _P, _I, _P, _ULL, _U, _P, _P]),
@@ -127,6 +155,11 @@ SIGNATURES = {
     'ultr_clip_adagrad2': (_I, [_P, _P, _P, _LL, _P, _F, _F, _F, _F, _I, _P, _P, _P, _P, _P, _I, _P, _F, _F, _F, _F, _P, _P]),
     'ultr_clip_adagrad3': (_I, [_P, _P, _P, _LL, _P, _F, _F, _F, _F, _I, _P, _P, _P, _P, _P, _I, _P, _F, _F, _F, _F, _P,
                                 _P, _I, _LL, _P, _P, _I, _P]),
+    'ultr_tensors_table_bytes': (_LL, [_TENSOR, _I]),
+    'ultr_tensors_plan': (_I, [_TENSOR, _I, _P, _LL, _PLAN, _P]),
+    'ultr_global_norm': (_I, [_PLAN, _P, _F, _P, _P]),
+    'ultr_clip_by_global_norm': (_I, [_PLAN, _P, _F, _F, _P, _P]),
+    'ultr_clip_adagrad_tensors': (_I, [_PLAN, _P, _F, _F, _F, _F, _I, _P, _P]),
 }
 
 _lib = None

@@ -1,4 +1,5 @@
 from .base_algorithm import BaseAlgorithm
+from .gradient_tensors import GradientTensors
 from .dla import DLA
 from .ipw_rank import IPWrank
 from .regression_EM import RegressionEM

@@ -1,0 +1,130 @@
+"""Global gradient norm, clipping and the Adagrad / SGD update over many separate tensors.
+
+Reference: tf.clip_by_global_norm + optimizer.apply_gradients over the list of trainable variables (dla.py:237-255,
+ipw_rank.py:155-165).  The learning algorithms of this package keep their variables in one flat float32 buffer
+(``ultr_clip_adagrad``); a model whose parameters are tensors of their own lists them here, once.
+"""
+import ctypes
+
+import torch
+
+from .. import _lib
+
+_DTYPE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_STRATEGY = {'ada': _lib.OPT_ADAGRAD, 'sgd': _lib.OPT_SGD}  # the grad_strategy hparam
+
+
+class GradientTensors(object):
+    """A list of gradients (float32, bfloat16, float16, mixed as they come) and what belongs to them.
+
+    grads    tensors of any shape, contiguous; a tensor without elements is allowed
+    out      where ``clip`` writes, one per gradient and of its type; default: new tensors; pass ``grads`` to clip in place
+    params   float32, one per gradient: what ``clip_adagrad`` updates
+    accums   float32: Adagrad's accumulators (the reference starts them at 0.1)
+    copies   bfloat16 / float16 / float32: rewritten from the updated parameters; entries may be None
+
+    The constructor lays the list out on the device and waits for that; it cannot be captured into a graph.  The tensors
+    are held and their CURRENT values are read by every call.  The calls enqueue on torch's current stream, allocate
+    nothing once ``out`` is there, never synchronise, and may be captured.  Calls on one object (and replays of graphs that
+    captured them) must be ordered one after the other: they share its partial sums."""
+
+    def __init__(self, grads, out=None, params=None, accums=None, copies=None):
+        if not torch.cuda.is_available():
+            raise _lib.UltrError('GradientTensors needs an MI355X (HIP) device: there is no CPU path')
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('GradientTensors lays its list out on the device: build it before the capture')
+        self.grads = list(grads)
+        self.device = torch.device('cuda', torch.cuda.current_device())
+        self.params, self.accums, self.copies = (None if v is None else list(v) for v in (params, accums, copies))
+        self.out = None if out is None else list(out)
+        for name, want in (('out', None), ('params', torch.float32), ('accums', torch.float32), ('copies', False)):
+            self._check_role(name, want)
+        for k, g in enumerate(self.grads):
+            if g.dtype not in _DTYPE or g.device != self.device or not g.is_contiguous():
+                raise ValueError('grads[%d]: a contiguous float32, bfloat16 or float16 tensor on %s expected, got %s on %s'
+                                 % (k, self.device, g.dtype, g.device))
+        self.norm = torch.zeros(1, dtype=torch.float32, device=self.device)
+        self._build()
+
+    def _check_role(self, name, dtype):
+        tensors = getattr(self, name)
+        if tensors is None:
+            return
+        if len(tensors) != len(self.grads):
+            raise ValueError('%s: %d tensors for %d gradients' % (name, len(tensors), len(self.grads)))
+        for k, (t, g) in enumerate(zip(tensors, self.grads)):
+            if t is None and dtype is False:
+                continue
+            ok = t.dtype in _DTYPE if dtype is False else t.dtype == (g.dtype if dtype is None else dtype)
+            if not ok or t.shape != g.shape or t.device != self.device or not t.is_contiguous():
+                raise ValueError('%s[%d]: contiguous %s %s on %s expected, got %s %s on %s'
+                                 % (name, k, dtype or g.dtype, tuple(g.shape), self.device, t.dtype, tuple(t.shape), t.device))
+
+    def _build(self):
+        n = len(self.grads)
+        rec = (_lib.UltrTensor * max(n, 1))()
+        for k, g in enumerate(self.grads):
+            r = rec[k]
+            r.grad, r.n, r.grad_dtype = g.data_ptr(), g.numel(), _DTYPE[g.dtype]
+            if self.out is not None:
+                r.out = self.out[k].data_ptr()
+            if self.params is not None:
+                r.param = self.params[k].data_ptr()
+            if self.accums is not None:
+                r.accum = self.accums[k].data_ptr()
+            if self.copies is not None and self.copies[k] is not None:
+                r.copy, r.copy_dtype = self.copies[k].data_ptr(), _DTYPE[self.copies[k].dtype]
+        lib = _lib.lib()
+        nbytes = lib.ultr_tensors_table_bytes(rec, n)
+        if nbytes < 0:
+            raise _lib.UltrError(lib.ultr_last_error().decode())
+        self._table = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        self._plan = _lib.UltrTensorPlan()
+        _lib.check(lib.ultr_tensors_plan(rec, n, _lib.ptr(self._table), nbytes, self._plan, _lib.current_stream()),
+                   'ultr_tensors_plan')
+        # whichever stream uses the plan later finds it written
+        torch.cuda.current_stream().synchronize()
+
+    def _stream(self):
+        if torch.cuda.current_device() != self.device.index:
+            raise ValueError('these tensors live on %s, the current device is cuda:%d' % (self.device, torch.cuda.current_device()))
+        return _lib.current_stream()
+
+    def _denom(self, denom):
+        if denom is None:
+            return None
+        if denom.device != self.device or denom.dtype != torch.float32 or denom.numel() < 1:
+            raise ValueError('denom: a float32 device scalar expected')
+        return denom.data_ptr()
+
+    def global_norm(self, denom=None, scale=1.0):
+        """sqrt of the sum over all gradients of (scale / denom * g)^2, a device tensor [1] that the next call overwrites."""
+        _lib.check(_lib.lib().ultr_global_norm(self._plan, self._denom(denom), scale, self.norm.data_ptr(), self._stream()),
+                   'ultr_global_norm')
+        return self.norm
+
+    def clip(self, clip_norm, denom=None, scale=1.0):
+        """-> (out, norm), as tf.clip_by_global_norm: out = scale / denom * g * clip_norm / max(norm, clip_norm).  A norm that
+        is not finite makes every output NaN; clip_norm <= 0 does not clip."""
+        if self.out is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError('clip: give ``out`` to the constructor before capturing')
+            self.out = [torch.empty_like(g) for g in self.grads]
+            self._build()
+        _lib.check(_lib.lib().ultr_clip_by_global_norm(self._plan, self._denom(denom), scale, clip_norm,
+                                                       self.norm.data_ptr(), self._stream()), 'ultr_clip_by_global_norm')
+        return self.out, self.norm
+
+    def clip_adagrad(self, clip_norm, learning_rate, denom=None, scale=1.0, l2=0.0, grad_strategy='ada'):
+        """Clip and update the parameters in place (and the accumulators, and the copies); the gradients stay as they are.
+        e = scale / denom * g + l2 * param; the norm is over e.  grad_strategy: 'ada' or 'sgd', as the hparam.
+        -> norm, a device tensor [1] that the next call overwrites."""
+        if self.params is None:
+            raise ValueError('clip_adagrad: the list was built without params')
+        strategy = _STRATEGY.get(grad_strategy)
+        if strategy is None:
+            raise ValueError("grad_strategy '%s' unknown (ada, sgd)" % grad_strategy)
+        _lib.check(_lib.lib().ultr_clip_adagrad_tensors(self._plan, self._denom(denom), scale, l2, clip_norm, learning_rate,
+                                                        strategy, self.norm.data_ptr(), self._stream()),
+                   'ultr_clip_adagrad_tensors')
+        return self.norm
