@@ -269,7 +269,7 @@ int ultr_layer_norm_forward(const void* x, long long ldx, const void* gamma, con
  * dx, d_gamma and d_beta may each be NULL (not wanted), not all of them.  dx must not overlap x or dy.
  * The sums over rows are fp32 in an order that depends on (M, N, types) only: equal calls give equal bits.
  * ws: ultr_layer_norm_workspace_bytes(M, N) bytes, 16-byte aligned, contents irrelevant before and after the call; may
- * be NULL when that is 0 or when neither d_gamma nor d_beta is wanted.  Two calls in flight need a workspace each. */
+ * be NULL when that is 0, or for dx alone at N <= 8192.  Two calls in flight need a workspace each. */
 long long ultr_layer_norm_workspace_bytes(long long M, int N);
 int ultr_layer_norm_backward(const void* dy, long long lddy, const void* x, long long ldx, const float* stats,
                              const void* gamma, long long M, int N, int x_dtype, int w_dtype, void* dx, long long lddx,

@@ -296,6 +296,19 @@ def test_rows_beyond_32_bit_offsets():
     assert torch.equal(out, y)
 
 
+def test_more_rows_than_one_grid_takes():
+    from ultra_amd.ranking_model import layer_norm
+    m = (1 << 27) + (1 << 20) + 5
+    x = torch.randn((m, 2), device='cuda', dtype=torch.float16)
+    y, stats = layer_norm(x)
+    for at in (0, (1 << 27) - 300, m - 300):
+        part = slice(at, min(m, at + 700))
+        ry, rs, ty, ts = ref_forward(x[part], None, None)
+        within(y[part], ry, ty, 'y')
+        within(stats[part], rs, ts, 'stats')
+    assert torch.isfinite(stats).all()
+
+
 def test_streams_and_workspaces():
     """Two backward passes in flight, each with its own workspace, on streams of their own."""
     from ultra_amd.ranking_model import layer_norm, layer_norm_backward, layer_norm_workspace

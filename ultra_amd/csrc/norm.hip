@@ -3,98 +3,81 @@
 //   forward   mu = sum x / N ; v = sum (x - mu)^2 / N ; r = 1 / sqrt(v + eps) ; y = (x - mu) r gamma + beta
 //   backward  xh = (x - mu) r ; g = dy gamma ; dx = r (g - sum g / N - xh sum(g xh) / N)
 //             d_gamma = sum_m dy xh ; d_beta = sum_m dy
-#include "storage.hpp"
+#include "norm_body.hpp"
 
 #include <algorithm>
 #include <type_traits>
 
 namespace ultr {
 
-constexpr int kNThreads = 256;
-constexpr int kNMaxSlices = 64;
-
-template <typename T, typename W>
-__global__ void __launch_bounds__(kNThreads) layer_norm_kernel(const T* x, long long ldx, const W* gamma, const W* beta,
-                                                               long long M, int N, float eps, T* y, long long ldy,
-                                                               float* stats) {
-  __shared__ float red[kNThreads / 64];
-  for (long long m = blockIdx.x; m < M; m += gridDim.x) {
-    const T* xr = x + m * ldx;
-    T* yr = y + m * ldy;
-    float s[1] = {0.f};
-    for (int i = threadIdx.x; i < N; i += kNThreads) s[0] += to_f32(xr[i]);
-    block_sum<1>(s, red);
-    const float mean = s[0] / N;
-    s[0] = 0.f;
-    for (int i = threadIdx.x; i < N; i += kNThreads) {
-      const float d = to_f32(xr[i]) - mean;
-      s[0] = fmaf(d, d, s[0]);
-    }
-    block_sum<1>(s, red);
-    const float rstd = 1.f / sqrtf(s[0] / N + eps);
-    for (int i = threadIdx.x; i < N; i += kNThreads)
-      yr[i] = from_f32<T>(fmaf((to_f32(xr[i]) - mean) * rstd, gamma ? to_f32(gamma[i]) : 1.f, beta ? to_f32(beta[i]) : 0.f));
-    if (threadIdx.x == 0 && stats) {
-      stats[2 * m] = mean;
-      stats[2 * m + 1] = rstd;
-    }
+// ---- which threads hold a row ------------------------------------------------------------------------------------------
+template <int TPR_, int C_, int V_>
+struct Shape {
+  static constexpr int TPR = TPR_, C = C_, V = V_;
+};
+// The first of the shapes that holds N entries.
+template <typename... S, typename F>
+static void first_shape(int N, F&& fn, S... shapes) {
+  (void)((N <= S::TPR * S::C * S::V ? (fn(shapes), true) : false) || ...);
+}
+// Forward: 8 elements a thread until a workgroup is full (two 16-byte pieces of fp32, one of 16-bit types; with 4 or 16 the
+// same widths lose 2 to 10 %), then more.  Rows shorter than one piece: element by element.
+template <typename T, typename F>
+static void forward_shape(int N, F&& fn) {
+  if constexpr (sizeof(T) == 4) {
+    if (N < 4) return fn(Shape<4, 1, 1>{});
+    first_shape(N, fn, Shape<4, 1, 4>{}, Shape<8, 2, 4>{}, Shape<16, 2, 4>{}, Shape<32, 2, 4>{}, Shape<64, 2, 4>{}, Shape<128, 2, 4>{},
+                Shape<256, 2, 4>{}, Shape<512, 2, 4>{}, Shape<1024, 2, 4>{}, Shape<1024, 4, 4>{}, Shape<1024, 8, 4>{},
+                Shape<1024, 16, 4>{});
+  } else {
+    if (N < 8) return fn(Shape<8, 1, 1>{});
+    first_shape(N, fn, Shape<4, 1, 8>{}, Shape<8, 1, 8>{}, Shape<16, 1, 8>{}, Shape<32, 1, 8>{}, Shape<64, 1, 8>{}, Shape<128, 1, 8>{},
+                Shape<256, 1, 8>{}, Shape<512, 1, 8>{}, Shape<512, 2, 8>{}, Shape<1024, 2, 8>{}, Shape<1024, 4, 8>{},
+                Shape<1024, 8, 8>{});
+  }
+}
+// Backward: 16 elements a thread, up to the 512 threads of a workgroup.
+constexpr int kGradWidth = 16 * kGradThreads;
+template <typename T, typename F>
+static void grad_shape(int N, F&& fn) {
+  if constexpr (sizeof(T) == 4) {
+    if (N < 4) return fn(Shape<4, 1, 1>{});
+    first_shape(N, fn, Shape<4, 1, 4>{}, Shape<4, 4, 4>{}, Shape<8, 4, 4>{}, Shape<16, 4, 4>{}, Shape<32, 4, 4>{}, Shape<64, 4, 4>{},
+                Shape<128, 4, 4>{}, Shape<256, 4, 4>{}, Shape<512, 4, 4>{});
+  } else {
+    if (N < 8) return fn(Shape<8, 1, 1>{});
+    first_shape(N, fn, Shape<4, 1, 8>{}, Shape<4, 2, 8>{}, Shape<8, 2, 8>{}, Shape<16, 2, 8>{}, Shape<32, 2, 8>{}, Shape<64, 2, 8>{},
+                Shape<128, 2, 8>{}, Shape<256, 2, 8>{}, Shape<512, 2, 8>{});
   }
 }
 
-template <typename T, typename W>
-__global__ void __launch_bounds__(kNThreads) layer_norm_dx_kernel(const T* dy, long long lddy, const T* x, long long ldx,
-                                                                  const float* stats, const W* gamma, long long M, int N,
-                                                                  T* dx, long long lddx) {
-  __shared__ float red[2 * kNThreads / 64];
-  for (long long m = blockIdx.x; m < M; m += gridDim.x) {
-    const T* xr = x + m * ldx;
-    const T* dr = dy + m * lddy;
-    const float mean = stats[2 * m], rstd = stats[2 * m + 1];
-    float s[2] = {0.f, 0.f};
-    for (int i = threadIdx.x; i < N; i += kNThreads) {
-      const float g = to_f32(dr[i]) * (gamma ? to_f32(gamma[i]) : 1.f);
-      s[0] += g;
-      s[1] = fmaf(g, (to_f32(xr[i]) - mean) * rstd, s[1]);
-    }
-    block_sum<2>(s, red);
-    const float a = s[0] / N, b = s[1] / N;
-    for (int i = threadIdx.x; i < N; i += kNThreads) {
-      const float g = to_f32(dr[i]) * (gamma ? to_f32(gamma[i]) : 1.f);
-      dx[m * lddx + i] = from_f32<T>(rstd * (g - a - (to_f32(xr[i]) - mean) * rstd * b));
-    }
-  }
+// Workgroups of the backward pass that holds rows = partial rows of d_gamma and d_beta, for row groups of `rg` rows.  One per
+// CU; half of them while each would get fewer than 3 turns (the partial rows cost more than the idle CUs: 1000 rows of 4096
+// bf16 14.3 us with 128, 15.4 with 256; 3000 rows 25.4 and 22.1).  Up to 4 turns one workgroup does it all: no second launch.
+static int grad_blocks(long long M, int rg) {
+  const long long turns = cdiv(M, rg);
+  if (turns <= 4) return 1;
+  return (int)std::min<long long>(turns, turns < 3 * 256 ? 128 : 256);
+}
+static int grad_row_groups(int N, int x_dtype) {
+  int rg = 1;
+  auto set = [&](auto s) { rg = kGradThreads / decltype(s)::TPR; };
+  if (x_dtype == ULTR_DTYPE_F32) grad_shape<float>(N, set);
+  else grad_shape<bf16_t>(N, set);
+  return rg;
+}
+// Row slices of the wide pass: about 512 workgroups, at least 4 rows each; a multiple of 8 (see the kernel) unless that few.
+static int wide_slices(long long M, int N, int x_dtype) {
+  const int tiles = (int)cdiv(N, kNThreads * (x_dtype == ULTR_DTYPE_F32 ? 4 : 8));
+  const long long s = std::min<long long>((512 / tiles + 7) / 8 * 8, M / 4);
+  return (int)(s < 8 ? std::max<long long>(s, 1) : s / 8 * 8);
+}
+static int partial_rows(long long M, int N, int x_dtype) {
+  return N <= kGradWidth ? grad_blocks(M, grad_row_groups(N, x_dtype)) : wide_slices(M, N, x_dtype);
 }
 
-// Column sums of one slice of rows: ws[slice][0][N] of dy * xh, ws[slice][1][N] of dy.
-template <typename T>
-__global__ void __launch_bounds__(kNThreads) layer_norm_dw_kernel(const T* dy, long long lddy, const T* x, long long ldx,
-                                                                  const float* stats, long long M, int N, float* ws) {
-  const int i = blockIdx.x * kNThreads + threadIdx.x;
-  if (i >= N) return;
-  float dg = 0.f, db = 0.f;
-  for (long long m = blockIdx.y; m < M; m += gridDim.y) {
-    const float d = to_f32(dy[m * lddy + i]);
-    dg = fmaf(d, (to_f32(x[m * ldx + i]) - stats[2 * m]) * stats[2 * m + 1], dg);
-    db += d;
-  }
-  float* w = ws + (long long)blockIdx.y * 2 * N;
-  w[i] = dg;
-  w[N + i] = db;
-}
-template <typename W>
-__global__ void __launch_bounds__(kNThreads) layer_norm_dw_sum_kernel(const float* ws, int slices, int N, W* d_gamma, W* d_beta) {
-  const int i = blockIdx.x * kNThreads + threadIdx.x;
-  if (i >= N) return;
-  float dg = 0.f, db = 0.f;
-  for (int s = 0; s < slices; ++s) {
-    dg += ws[(long long)s * 2 * N + i];
-    db += ws[(long long)s * 2 * N + N + i];
-  }
-  if (d_gamma) d_gamma[i] = from_f32<W>(dg);
-  if (d_beta) d_beta[i] = from_f32<W>(db);
-}
-
-static int slices_of(long long M) { return (int)std::min<long long>(M, kNMaxSlices); }
+// One grid holds fewer than 2^32 threads: longer matrices go in slabs of whole workgroups.
+constexpr long long kSlabBlocks = 1ll << 21;
 
 // Calls fn with null pointers of the storage types: fn(T*, W*).
 template <typename F>
@@ -103,6 +86,19 @@ static int with_types(int x_dtype, int w_dtype, F&& fn) {
   if (x_dtype == ULTR_DTYPE_BF16)
     return w_dtype == ULTR_DTYPE_F32 ? fn((bf16_t*)nullptr, (float*)nullptr) : fn((bf16_t*)nullptr, (bf16_t*)nullptr);
   return w_dtype == ULTR_DTYPE_F32 ? fn((f16_t*)nullptr, (float*)nullptr) : fn((f16_t*)nullptr, (f16_t*)nullptr);
+}
+
+template <typename W>
+static int launch_dw_sum(const float* part, int parts, int N, W* d_gamma, W* d_beta, hipStream_t s) {
+  {
+    ProfScope prof_("layer_norm_dw_sum_kernel", s);
+    const unsigned grid = (unsigned)cdiv(2 * N, 32);
+    if (parts > 64)
+      hipLaunchKernelGGL((layer_norm_dw_sum_kernel<W, 32>), dim3(grid), dim3(1024), 0, s, part, parts, N, d_gamma, d_beta);
+    else
+      hipLaunchKernelGGL((layer_norm_dw_sum_kernel<W, 8>), dim3(grid), dim3(256), 0, s, part, parts, N, d_gamma, d_beta);
+  }
+  return check_launch("layer_norm_dw_sum_kernel");
 }
 
 static int check_norm(const char* who, long long M, int N, int x_dtype, int w_dtype) {
@@ -145,23 +141,49 @@ extern "C" int ultr_layer_norm_forward(const void* x, long long ldx, const void*
   ULTR_REQUIRE((x == y && (ldx == ldy || M <= 1)) || !rows_overlap(x, ldx, y, ldy, M, N, x_dtype), ULTR_EINVAL,
                "%s: y overlaps x without being x", who);
   if (M == 0) return ULTR_OK;
-  const unsigned grid = (unsigned)std::min<long long>(M, 65536);
-  {
-    ProfScope prof_("layer_norm_kernel", as_stream(stream));
-    with_types(x_dtype, w_dtype, [&](auto* t, auto* w) {
-      using T = std::remove_pointer_t<decltype(t)>;
-      using W = std::remove_pointer_t<decltype(w)>;
-      hipLaunchKernelGGL((layer_norm_kernel<T, W>), dim3(grid), dim3(kNThreads), 0, as_stream(stream), (const T*)x, ldx,
-                         (const W*)gamma, (const W*)beta, M, N, eps, (T*)y, ldy, stats);
-      return 0;
+  hipStream_t s = as_stream(stream);
+  const float inv_n = 1.f / (float)N;
+  with_types(x_dtype, w_dtype, [&](auto* t, auto* w) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    using W = std::remove_pointer_t<decltype(w)>;
+    forward_shape<T>(N, [&](auto shape) {
+      using S = decltype(shape);
+      constexpr int NT = S::TPR < 256 ? 256 : S::TPR;
+      auto go = [&](auto tail, auto r) {
+        constexpr int R = decltype(r)::value;
+        constexpr long long rows = (long long)R * (NT / S::TPR);
+        for (long long m = 0; m < M; m += kSlabBlocks * rows) {
+          const long long n = std::min(M - m, kSlabBlocks * rows);
+          ProfScope prof_("layer_norm_kernel", s);
+          hipLaunchKernelGGL((layer_norm_kernel<T, W, S::TPR, S::C, S::V, decltype(tail)::value, R>), dim3((unsigned)cdiv(n, rows)),
+                             dim3(NT), 0, s, (const T*)x + m * ldx, ldx, (const W*)gamma, (const W*)beta, n, N, inv_n, eps,
+                             (T*)y + m * ldy, ldy, stats ? stats + 2 * m : nullptr);
+        }
+      };
+      // two rows a thread group once there are rows enough to fill the chip that way (512 rows of 4096 bf16: 4.5 us with
+      // one, 4.8 with two; 4096 rows: 18.1 and 16.4), and registers for both
+      constexpr bool pair = S::C * S::V * sizeof(T) <= 64;
+      auto rows = [&](auto tail) {
+        if constexpr (pair) {
+          if (M >= 2048) return go(tail, std::integral_constant<int, 2>{});
+        }
+        go(tail, std::integral_constant<int, 1>{});
+      };
+      if (S::V > 1 && N % S::V) rows(std::integral_constant<bool, (S::V > 1)>{});
+      else rows(std::false_type{});
     });
-  }
+    return 0;
+  });
   return check_launch("layer_norm_kernel");
 }
 
+// Partial rows of d_gamma and d_beta, behind the row sums of the wide pass.  The types share one size: the larger.
+static long long sums_bytes(long long M, int N) { return N <= kGradWidth ? 0 : (M * 8 + 15) / 16 * 16; }
 extern "C" long long ultr_layer_norm_workspace_bytes(long long M, int N) {
   if (check_norm("ultr_layer_norm_workspace_bytes", M, N, ULTR_DTYPE_F32, ULTR_DTYPE_F32) != ULTR_OK) return -1;
-  return (long long)slices_of(M) * 2 * N * (long long)sizeof(float);
+  if (M == 0) return 0;
+  const long long p = std::max(partial_rows(M, N, ULTR_DTYPE_F32), partial_rows(M, N, ULTR_DTYPE_BF16));
+  return sums_bytes(M, N) + (p > 1 ? p * 2 * N * (long long)sizeof(float) : 0);
 }
 
 extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const void* x, long long ldx, const float* stats,
@@ -181,37 +203,54 @@ extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const vo
   ULTR_REQUIRE(!rows_overlap(dx, lddx, x, ldx, M, N, x_dtype) && !rows_overlap(dx, lddx, dy, lddy, M, N, x_dtype), ULTR_EINVAL,
                "%s: dx overlaps x or dy", who);
   const bool dw = d_gamma || d_beta;
-  ULTR_REQUIRE(!dw || ws || ultr_layer_norm_workspace_bytes(M, N) == 0, ULTR_EINVAL, "%s: workspace required", who);
+  ULTR_REQUIRE((!dw && N <= kGradWidth) || ws || ultr_layer_norm_workspace_bytes(M, N) == 0, ULTR_EINVAL,
+               "%s: workspace required", who);
   hipStream_t s = as_stream(stream);
+  const float inv_n = 1.f / (float)N;
   return with_types(x_dtype, w_dtype, [&](auto* t, auto* w) {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
-    if (dx && M > 0) {
-      {
-        ProfScope prof_("layer_norm_dx_kernel", s);
-        hipLaunchKernelGGL((layer_norm_dx_kernel<T, W>), dim3((unsigned)std::min<long long>(M, 65536)), dim3(kNThreads), 0, s,
-                           (const T*)dy, lddy, (const T*)x, ldx, stats, (const W*)gamma, M, N, (T*)dx, lddx);
-      }
-      const int rc2 = check_launch("layer_norm_dx_kernel");
-      if (rc2) return rc2;
+    if (M == 0) return launch_dw_sum(nullptr, 0, N, (W*)d_gamma, (W*)d_beta, s);
+    const int parts = partial_rows(M, N, x_dtype);
+    float* part = dw && parts > 1 ? (float*)((char*)ws + sums_bytes(M, N)) : nullptr;
+    W *dg = part ? nullptr : (W*)d_gamma, *db = part ? nullptr : (W*)d_beta;
+    if (N <= kGradWidth) {
+      grad_shape<T>(N, [&](auto shape) {
+        using S = decltype(shape);
+        auto go = [&](auto tail) {
+          ProfScope prof_("layer_norm_grad_kernel", s);
+          hipLaunchKernelGGL((layer_norm_grad_kernel<T, W, S::TPR, S::C, S::V, decltype(tail)::value>), dim3(parts),
+                             dim3(kGradThreads), 0, s, (const T*)dy, lddy, (const T*)x, ldx, stats, (const W*)gamma, M, N, inv_n,
+                             (T*)dx, lddx, part, dg, db);
+        };
+        if (S::V > 1 && N % S::V) go(std::integral_constant<bool, (S::V > 1)>{});
+        else go(std::false_type{});
+      });
+    } else {
+      constexpr int V = 16 / sizeof(T);
+      float2* sums = (float2*)ws;
+      auto go = [&](auto tail) {
+        constexpr bool TAIL = decltype(tail)::value;
+        if (dx) {
+          ProfScope prof_("layer_norm_row_sums_kernel", s);
+          // few rows: all the threads a workgroup can have; many: more rows at a time (4096 of 16384 bf16: 60 and 50 us)
+          const unsigned grid = (unsigned)std::min<long long>(M, 2048);
+          if (M >= 512)
+            hipLaunchKernelGGL((layer_norm_row_sums_kernel<T, W, V, TAIL, 256>), dim3(grid), dim3(256), 0, s, (const T*)dy, lddy,
+                               (const T*)x, ldx, stats, (const W*)gamma, M, N, inv_n, sums);
+          else
+            hipLaunchKernelGGL((layer_norm_row_sums_kernel<T, W, V, TAIL, 1024>), dim3(grid), dim3(1024), 0, s, (const T*)dy, lddy,
+                               (const T*)x, ldx, stats, (const W*)gamma, M, N, inv_n, sums);
+        }
+        ProfScope prof_("layer_norm_wide_grad_kernel", s);
+        hipLaunchKernelGGL((layer_norm_wide_grad_kernel<T, W, V, TAIL>), dim3(parts, (unsigned)cdiv(N, kNThreads * V)),
+                           dim3(kNThreads), 0, s, (const T*)dy, lddy, (const T*)x, ldx, stats, (const W*)gamma, sums, M, N, (T*)dx,
+                           lddx, part, dg, db);
+      };
+      if (N % V) go(std::true_type{});
+      else go(std::false_type{});
     }
-    if (!dw) return ULTR_OK;
-    const int slices = slices_of(M);
-    const unsigned gx = (unsigned)cdiv(N, kNThreads);
-    if (M > 0) {
-      {
-        ProfScope prof_("layer_norm_dw_kernel", s);
-        hipLaunchKernelGGL((layer_norm_dw_kernel<T>), dim3(gx, slices), dim3(kNThreads), 0, s, (const T*)dy, lddy, (const T*)x,
-                           ldx, stats, M, N, (float*)ws);
-      }
-      const int rc2 = check_launch("layer_norm_dw_kernel");
-      if (rc2) return rc2;
-    }
-    {
-      ProfScope prof_("layer_norm_dw_sum_kernel", s);
-      hipLaunchKernelGGL((layer_norm_dw_sum_kernel<W>), dim3(gx), dim3(kNThreads), 0, s, (const float*)ws, slices, N,
-                         (W*)d_gamma, (W*)d_beta);
-    }
-    return check_launch("layer_norm_dw_sum_kernel");
+    const int rc2 = check_launch("layer_norm_grad_kernel");
+    return rc2 || !part ? rc2 : launch_dw_sum(part, parts, N, (W*)d_gamma, (W*)d_beta, s);
   });
 }

@@ -1,0 +1,343 @@
+// Kernels of the stand-alone layer normalisation (norm.hip).
+#pragma once
+#include "storage.hpp"
+
+namespace ultr {
+
+constexpr int kNThreads = 256;
+constexpr int kGradThreads = 512;  // one workgroup a CU: 8 waves with up to 256 registers each
+
+// Sums over the TPR threads that share a row (a power of two: part of a wave, a wave, or whole waves of one workgroup); all
+// of them get the totals.  K values at once; red: K floats per wave of the workgroup.  The exchange ends without a barrier, so
+// the next one must use another `red`, and the one after that may use this again.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float* red) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = group_sum<(TPR < 64 ? TPR : 64)>(v[k]);
+  if (TPR > 64) {
+    const int wave = threadIdx.x >> 6, first = wave & ~(TPR / 64 - 1);
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[wave * K + k] = v[k];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < TPR / 64; ++w) v[k] += red[(first + w) * K + k];
+    }
+  }
+}
+
+// Where a thread's C pieces of V elements lie in a row of N.  With TAIL (N no multiple of V, N >= V) the last piece is moved
+// back to end with the row; its first skip[] elements belong to the piece before it as well: they are left out of sums, and
+// both pieces store the same values for them.  skip >= V: no piece.
+template <int TPR, int C, int V, bool TAIL>
+struct Pieces {
+  int at[C], skip[C];
+  __device__ __forceinline__ Pieces(int lane, int N) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int i = (c * TPR + lane) * V;
+      at[c] = TAIL ? min(i, N - V) : i;
+      skip[c] = TAIL ? i - at[c] : (i < N ? 0 : V);
+    }
+  }
+  __device__ __forceinline__ bool any(int c) const { return skip[c] < V; }
+  __device__ __forceinline__ float counted(int c, int j, float v) const { return !TAIL || j >= skip[c] ? v : 0.f; }
+};
+
+// Forward.  HBM-bound: one read and one write of the matrix.  TPR threads hold R whole rows in registers, so the mean, the
+// variance about it and the output need one pass over memory.  R = 2: the weights, which come out of the caches once per
+// row otherwise, serve two rows (fp16 rows of 5003 with fp32 weights, 30010 of them: 117 us against 158).  Narrow rows
+// ask for their weights along with the row (136 fp32: 5.0 TB/s against 4.3); in a workgroup of several waves the other
+// workgroups cover that latency and the registers are worth more (8192 fp32, R = 2: 5.6 TB/s against 4.7).
+template <typename T, typename W, int TPR, int C, int V, bool TAIL, int R>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
+    layer_norm_kernel(const T* x, long long ldx, const W* gamma, const W* beta, long long M, int N, float inv_n, float eps,
+                      T* y, long long ldy, float* stats) {
+  constexpr int NT = TPR < 256 ? 256 : TPR;
+  constexpr bool EARLY = TPR <= 128;
+  typedef typename Piece<T, V>::type PT;
+  typedef typename Piece<W, V>::type PW;
+  __shared__ float red[2][R * NT / 64];
+  const int lane = threadIdx.x % TPR;
+  const long long row0 = ((long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR) * R;
+  const Pieces<TPR, C, V, TAIL> pc(lane, N);
+  PT raw[R][C];
+  PW g[C], b[C];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const T* xr = x + min(row0 + r, M - 1) * ldx;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (pc.any(c)) raw[r][c] = *reinterpret_cast<const PT*>(xr + pc.at[c]);
+  }
+  auto weights = [&](int c) {
+    if (gamma) g[c] = *reinterpret_cast<const PW*>(gamma + pc.at[c]);
+    if (beta) b[c] = *reinterpret_cast<const PW*>(beta + pc.at[c]);
+  };
+  if (EARLY) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (pc.any(c)) weights(c);
+  }
+  float mean[R], rstd[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    mean[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (!pc.any(c)) continue;
+#pragma unroll
+      for (int j = 0; j < V; ++j) mean[r] += pc.counted(c, j, to_f32(raw[r][c][j]));
+    }
+  }
+  row_sums<TPR>(mean, red[0]);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    mean[r] *= inv_n;
+    rstd[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (!pc.any(c)) continue;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = to_f32(raw[r][c][j]) - mean[r];
+        rstd[r] = fmaf(d, pc.counted(c, j, d), rstd[r]);
+      }
+    }
+  }
+  row_sums<TPR>(rstd, red[1]);
+#pragma unroll
+  for (int r = 0; r < R; ++r) rstd[r] = 1.f / sqrtf(fmaf(rstd[r], inv_n, eps));
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (!pc.any(c)) continue;
+    if (!EARLY) weights(c);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (row0 + r >= M) break;
+      float v[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        v[j] = (to_f32(raw[r][c][j]) - mean[r]) * rstd[r];
+        if (gamma) v[j] *= to_f32(g[c][j]);
+        if (beta) v[j] += to_f32(b[c][j]);
+      }
+      store_piece<V>(y + (row0 + r) * ldy + pc.at[c], v);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (lane == 0 && stats && row0 + r < M) *reinterpret_cast<float2*>(stats + 2 * (row0 + r)) = make_float2(mean[r], rstd[r]);
+}
+
+// Backward, rows that a workgroup holds.  HBM-bound: two reads and one write of the matrix.  A workgroup walks over the rows,
+// kGradThreads / TPR at a time, with the next ones on their way while these are worked on; a thread keeps its columns' share
+// of d_gamma and d_beta in registers over the whole walk.  What the row groups of a workgroup hold meets in LDS at the end
+// and leaves as one partial row (or the result itself when there is one workgroup).  16 elements a thread and 512 threads:
+// 16384 rows of 4096 bf16 77 us = 5.2 TB/s; with 1024 threads the registers spill (102 us), without the prefetch 8192 rows
+// of 8192 take 100 us against 81.
+template <typename T, typename W, int TPR, int C, int V, bool TAIL>
+__global__ void __launch_bounds__(kGradThreads)
+    layer_norm_grad_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,
+                           long long M, int N, float inv_n, T* dx, long long lddx, float* ws, W* d_gamma, W* d_beta) {
+  constexpr int NT = kGradThreads, RG = NT / TPR;
+  typedef typename Piece<T, V>::type PT;
+  __shared__ float red[2][2 * NT / 64];
+  __shared__ __align__(16) float cols[NT * C * V];
+  const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const Pieces<TPR, C, V, TAIL> pc(lane, N);
+  const bool dw = ws || d_gamma || d_beta;
+  float g_w[C][V], acc_g[C][V], acc_b[C][V];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      g_w[c][j] = 1.f;
+      acc_g[c][j] = acc_b[c][j] = 0.f;
+    }
+    if (gamma && pc.any(c)) load_piece<V>(gamma + pc.at[c], g_w[c]);
+  }
+  const long long step = (long long)gridDim.x * RG;
+  long long row = (long long)blockIdx.x * RG + group;
+  PT nx[C], nd[C];
+  float2 nst;
+  auto fetch = [&](long long r) {
+    r = min(r, M - 1);
+    nst = *reinterpret_cast<const float2*>(stats + 2 * r);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (pc.any(c)) {
+        nx[c] = *reinterpret_cast<const PT*>(x + r * ldx + pc.at[c]);
+        nd[c] = *reinterpret_cast<const PT*>(dy + r * lddy + pc.at[c]);
+      }
+  };
+  fetch(row);
+  int odd = 0;
+  for (long long first = (long long)blockIdx.x * RG; first < M; first += step, row += step, odd ^= 1) {
+    PT px[C], pd[C];
+    const float mean = nst.x, rstd = nst.y;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      px[c] = nx[c];
+      pd[c] = nd[c];
+    }
+    if (first + step < M) fetch(row + step);
+    const bool live = row < M;
+    float s[2] = {0.f, 0.f};
+    float xh[C][V], gr[C][V];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (!pc.any(c)) continue;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = to_f32(pd[c][j]);
+        xh[c][j] = (to_f32(px[c][j]) - mean) * rstd;
+        gr[c][j] = d * g_w[c][j];
+        const float gc = pc.counted(c, j, gr[c][j]);
+        s[0] += gc;
+        s[1] = fmaf(gc, xh[c][j], s[1]);
+        if (live) {
+          acc_g[c][j] = fmaf(d, xh[c][j], acc_g[c][j]);
+          acc_b[c][j] += d;
+        }
+      }
+    }
+    if (dx) {
+      row_sums<TPR>(s, red[odd]);
+      const float a = s[0] * inv_n, b = s[1] * inv_n;
+      if (live) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          if (!pc.any(c)) continue;
+          float v[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = rstd * (gr[c][j] - fmaf(xh[c][j], b, a));
+          store_piece<V>(dx + row * lddx + pc.at[c], v);
+        }
+      }
+    }
+  }
+  if (!dw) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) cols[group * (TPR * C * V) + (c * TPR + lane) * V + j] = which ? acc_b[c][j] : acc_g[c][j];
+    __syncthreads();
+    W* out = which ? d_beta : d_gamma;
+    float* part = ws ? ws + ((long long)blockIdx.x * 2 + which) * N : nullptr;
+    for (int i = threadIdx.x; i < TPR * C * V; i += NT) {
+      const int piece = i / V * V, at = TAIL ? min(piece, N - V) : piece;
+      const int col = at + i % V;
+      if (col < piece || col >= N) continue;  // an element of the piece before, or none
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < RG; ++k) sum += cols[k * (TPR * C * V) + i];
+      if (part) part[col] = sum;
+      else if (out) out[col] = from_f32<W>(sum);
+    }
+  }
+}
+
+// Backward, rows wider than that: the two sums of every row first, then a pass in which a workgroup owns a column tile and
+// a slice of the rows.  Reads the matrices twice; nothing but the two sums crosses threads.  The slice is the fastest index
+// of that pass's grid and a multiple of 8, so that (workgroups go to the 8 XCDs in turn) an XCD meets the rows whose sums
+// it formed, the last ones first: its L2 may still hold them (4096 rows of 16384 bf16: 124 us, other orders 130).
+template <typename T, typename W, int V, bool TAIL, int NT>
+__global__ void __launch_bounds__(NT)
+    layer_norm_row_sums_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,
+                               long long M, int N, float inv_n, float2* sums) {
+  __shared__ float red[2][2 * NT / 64];
+  int odd = 0;
+  for (long long m = blockIdx.x; m < M; m += gridDim.x, odd ^= 1) {
+    const float2 st = *reinterpret_cast<const float2*>(stats + 2 * m);
+    float s[2] = {0.f, 0.f};
+#pragma unroll 4
+    for (int i = threadIdx.x * V; i < N; i += NT * V) {
+      const int at = TAIL ? min(i, N - V) : i;
+      float vx[V], vd[V], g[V];
+      load_piece<V>(x + m * ldx + at, vx);
+      load_piece<V>(dy + m * lddy + at, vd);
+      if (gamma) load_piece<V>(gamma + at, g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float gr = !TAIL || at + j >= i ? (gamma ? vd[j] * g[j] : vd[j]) : 0.f;
+        s[0] += gr;
+        s[1] = fmaf(gr, (vx[j] - st.x) * st.y, s[1]);
+      }
+    }
+    row_sums<NT>(s, red[odd]);
+    if (threadIdx.x == 0) sums[m] = make_float2(s[0] * inv_n, s[1] * inv_n);
+  }
+}
+template <typename T, typename W, int V, bool TAIL>
+__global__ void __launch_bounds__(kNThreads)
+    layer_norm_wide_grad_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,
+                                const float2* sums, long long M, int N, T* dx, long long lddx, float* ws, W* d_gamma, W* d_beta) {
+  const int i = (blockIdx.y * kNThreads + threadIdx.x) * V;
+  if (i >= N) return;
+  const int at = TAIL ? min(i, N - V) : i;
+  float g[V], acc_g[V], acc_b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    g[j] = 1.f;
+    acc_g[j] = acc_b[j] = 0.f;
+  }
+  if (gamma) load_piece<V>(gamma + at, g);
+#pragma unroll 2
+  for (long long m = blockIdx.x + (M - 1 - blockIdx.x) / gridDim.x * gridDim.x; m >= 0; m -= gridDim.x) {
+    const float2 st = *reinterpret_cast<const float2*>(stats + 2 * m);
+    float vx[V], vd[V];
+    load_piece<V>(x + m * ldx + at, vx);
+    load_piece<V>(dy + m * lddy + at, vd);
+    const float2 ab = dx ? sums[m] : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float xh = (vx[j] - st.x) * st.y;
+      acc_g[j] = fmaf(vd[j], xh, acc_g[j]);
+      acc_b[j] += vd[j];
+      vx[j] = st.y * (vd[j] * g[j] - fmaf(xh, ab.y, ab.x));
+    }
+    if (dx) store_piece<V>(dx + m * lddx + at, vx);
+  }
+  if (ws) {
+    float* part = ws + (long long)blockIdx.x * 2 * N + at;
+    store_piece<V>(part, acc_g);
+    store_piece<V>(part + N, acc_b);
+  } else {  // one slice
+    if (d_gamma) store_piece<V>(d_gamma + at, acc_g);
+    if (d_beta) store_piece<V>(d_beta + at, acc_b);
+  }
+}
+
+// Sums the partial rows [P][2][N]: 32 columns a workgroup, K threads a column, fixed order.
+template <typename W, int K>
+__global__ void __launch_bounds__(32 * K) layer_norm_dw_sum_kernel(const float* ws, int P, int N, W* d_gamma, W* d_beta) {
+  __shared__ float part[K][33];
+  const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + c;
+  float s = 0.f;
+  if (col < 2 * N) {
+#pragma unroll 4
+    for (int p = k; p < P; p += K) s += ws[(long long)p * 2 * N + col];
+  }
+  part[k][c] = s;
+  __syncthreads();
+  if (k > 0 || col >= 2 * N) return;
+  s = 0.f;
+#pragma unroll
+  for (int q = 0; q < K; ++q) s += part[q][c];
+  if (col < N) {
+    if (d_gamma) d_gamma[col] = from_f32<W>(s);
+  } else if (d_beta) {
+    d_beta[col - N] = from_f32<W>(s);
+  }
+}
+
+}  // namespace ultr

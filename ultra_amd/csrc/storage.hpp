@@ -13,6 +13,26 @@ __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <typename T>
 __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 
+// A 16-byte (or shorter) piece of a row.  Its address is only as aligned as an element: gfx950 loads and stores
+// dwords at any byte address, so rows of odd width or stride take the same wide accesses as aligned ones.
+template <typename T, int V>
+struct Piece {
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+template <int V, typename T>
+__device__ __forceinline__ void load_piece(const T* p, float (&v)[V]) {
+  const auto q = *reinterpret_cast<const typename Piece<T, V>::type*>(p);
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = to_f32(q[j]);
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_piece(T* p, const float (&v)[V]) {
+  typename Piece<T, V>::type q;
+#pragma unroll
+  for (int j = 0; j < V; ++j) q[j] = from_f32<T>(v[j]);
+  *reinterpret_cast<typename Piece<T, V>::type*>(p) = q;
+}
+
 static inline bool known_dtype(int d) { return d == ULTR_DTYPE_F32 || d == ULTR_DTYPE_BF16 || d == ULTR_DTYPE_F16; }
 static inline int dtype_bytes(int d) { return d == ULTR_DTYPE_F32 ? 4 : 2; }
 

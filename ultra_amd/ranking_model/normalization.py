@@ -140,8 +140,8 @@ def layer_norm_backward(d_out, x, stats, gamma=None, d_x=None, d_gamma=None, d_b
     if need_g:
         w = _weight(d_gamma, 'd_gamma', x, w)
     ws = None
-    if need_g or need_b:
-        n = x.shape[-1]
+    n = x.shape[-1]
+    if need_g or need_b or n > 8192:
         if workspace is None:
             workspace = layer_norm_workspace(m, n, x.device)
         elif workspace.device != x.device or not workspace.is_contiguous() or \
