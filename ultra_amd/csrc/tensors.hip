@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 namespace ultr {
@@ -15,48 +16,48 @@ constexpr int kTThreads = 256;
 constexpr int kChunk = 4096;       // elements of one tensor that one workgroup takes at a time
 constexpr int kTMaxBlocks = 2048;  // workgroups of a pass, and partial sums of a norm
 
-struct TensorRec {  // UltrTensor as the kernels read it
+struct ChunkRec {  // what one chunk needs: its tensor's pointers, moved to its first element
   const void* grad;
   void* out;
   float* param;
   float* accum;
   void* copy;
-  long long n;
-  int grad_dtype, copy_dtype;
+  int n;
+  short grad_dtype, copy_dtype;
 };
-static_assert(sizeof(TensorRec) == sizeof(UltrTensor), "the table holds the caller's records");
+static_assert(sizeof(ChunkRec) == 48, "read as 12 words");
 
-// Table: records | chunk map (tensor, chunk within it) | partial sums of the norm.
-struct TableLayout {
-  long long map, partials, bytes;
-};
-static TableLayout table_layout(int n_tensors, long long n_chunks) {
-  TableLayout t;
-  t.map = (long long)n_tensors * sizeof(TensorRec);
-  t.partials = (t.map + n_chunks * (long long)sizeof(uint2) + 15) / 16 * 16;
-  t.bytes = t.partials + kTMaxBlocks * (long long)sizeof(double);
-  return t;
-}
+// Table: partial sums of the norm | a record per chunk.  One dependent load from a workgroup's number to its data; 48 bytes
+// for the 8 KB or more that a full chunk moves.
+constexpr long long kPartialBytes = kTMaxBlocks * sizeof(double);
+static long long table_bytes_of(long long n_chunks) { return kPartialBytes + n_chunks * (long long)sizeof(ChunkRec); }
 
 struct ListView {
-  const TensorRec* recs;
-  const uint2* map;
   double* partials;
+  const ChunkRec* chunks;
   long long n_chunks;
 };
 
-constexpr int kFillTensors = 48;  // records per fill launch: they travel as kernel arguments (3.5 KB)
+constexpr int kFillTensors = 48;  // tensors per fill launch: they travel as kernel arguments (3.5 KB)
 struct FillArgs {
-  TensorRec rec[kFillTensors];
+  UltrTensor t[kFillTensors];
   long long first_chunk[kFillTensors];
-  int first_tensor, count;
 };
-__global__ void __launch_bounds__(kTThreads) tensors_fill_kernel(FillArgs a, TensorRec* recs, uint2* map) {
-  for (int t = blockIdx.x; t < a.count; t += gridDim.x) {
-    if (threadIdx.x == 0 && blockIdx.y == 0) recs[a.first_tensor + t] = a.rec[t];
-    const long long chunks = (a.rec[t].n + kChunk - 1) / kChunk;
-    for (long long c = (long long)blockIdx.y * blockDim.x + threadIdx.x; c < chunks; c += (long long)gridDim.y * blockDim.x)
-      map[a.first_chunk[t] + c] = make_uint2((unsigned)(a.first_tensor + t), (unsigned)c);
+__global__ void __launch_bounds__(kTThreads) tensors_fill_kernel(FillArgs a, ChunkRec* chunks) {
+  const UltrTensor t = a.t[blockIdx.x];
+  const int g = t.grad_dtype == ULTR_DTYPE_F32 ? 4 : 2, cp = t.copy_dtype == ULTR_DTYPE_F32 ? 4 : 2;
+  for (long long c = (long long)blockIdx.y * blockDim.x + threadIdx.x; c * kChunk < t.n; c += (long long)gridDim.y * blockDim.x) {
+    const long long i = c * kChunk;
+    ChunkRec r;
+    r.grad = (const char*)t.grad + i * g;
+    r.out = t.out ? (char*)t.out + i * g : nullptr;
+    r.param = t.param ? t.param + i : nullptr;
+    r.accum = t.accum ? t.accum + i : nullptr;
+    r.copy = t.copy ? (char*)t.copy + i * cp : nullptr;
+    r.n = (int)min(t.n - i, (long long)kChunk);
+    r.grad_dtype = (short)t.grad_dtype;
+    r.copy_dtype = (short)t.copy_dtype;
+    chunks[a.first_chunk[blockIdx.x] + c] = r;
   }
 }
 
@@ -72,15 +73,22 @@ __device__ __forceinline__ double block_sum_f64(double v, double* red) {
   return s;
 }
 
-__device__ __forceinline__ float load_elem(const void* p, int dtype, long long i) {
-  if (dtype == ULTR_DTYPE_F32) return static_cast<const float*>(p)[i];
-  if (dtype == ULTR_DTYPE_BF16) return to_f32(static_cast<const bf16_t*>(p)[i]);
-  return to_f32(static_cast<const f16_t*>(p)[i]);
-}
-__device__ __forceinline__ void store_elem(void* p, int dtype, long long i, float v) {
-  if (dtype == ULTR_DTYPE_F32) static_cast<float*>(p)[i] = v;
-  else if (dtype == ULTR_DTYPE_BF16) static_cast<bf16_t*>(p)[i] = from_f32<bf16_t>(v);
-  else static_cast<f16_t*>(p)[i] = from_f32<f16_t>(v);
+// A chunk as a workgroup walks it, in pieces of V elements: all of a thread's pieces are loaded before the first is stored
+// (memory that may be the same for all the compiler knows keeps its order), in chunks that are not full too.  What is left
+// beyond whole pieces goes element by element to the last threads, whose wave has the least else to do there.
+// fn(at, ok, pieces, width): handle the pieces k of `width` elements at at(k) for which ok(k).
+template <int V, typename F>
+__device__ __forceinline__ void walk_chunk(int n, F&& fn) {
+  constexpr std::integral_constant<int, kChunk / (V * kTThreads)> pieces{};
+  constexpr std::integral_constant<int, V> width{};
+  auto at = [&](int k) { return (k * kTThreads + (int)threadIdx.x) * V; };
+  if (n == kChunk) {
+    fn(at, [](int) { return true; }, pieces, width);
+  } else {
+    fn(at, [&](int k) { return at(k) + V <= n; }, pieces, width);
+    const int rest = n % V, j = kTThreads - 1 - (int)threadIdx.x;
+    if (j < rest) fn([&](int) { return n - rest + j; }, [](int) { return true; }, std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
+  }
 }
 
 __device__ __forceinline__ float scale_of(const float* denom, float scale_const) {
@@ -96,20 +104,80 @@ __device__ __forceinline__ float clip_factor(double sumsq, float clip_norm, floa
   return n > (double)clip_norm ? (float)((double)clip_norm / n) : 1.f;
 }
 
+// fn(T*) for a storage type; it is the same for a whole chunk, so this is a scalar branch.
+template <typename F>
+__device__ __forceinline__ void with_type(int dtype, F&& fn) {
+  if (dtype == ULTR_DTYPE_F32) fn((float*)nullptr);
+  else if (dtype == ULTR_DTYPE_BF16) fn((bf16_t*)nullptr);
+  else fn((f16_t*)nullptr);
+}
+
+// A record read by the whole wave: the same for every lane, kept in scalar registers.
+__device__ __forceinline__ ChunkRec record_of(const ChunkRec* p) {
+  union {
+    ChunkRec r;
+    unsigned w[12];
+  } u;
+  const uint4* q = reinterpret_cast<const uint4*>(p);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const uint4 v = q[i];
+    u.w[4 * i] = __builtin_amdgcn_readfirstlane(v.x);
+    u.w[4 * i + 1] = __builtin_amdgcn_readfirstlane(v.y);
+    u.w[4 * i + 2] = __builtin_amdgcn_readfirstlane(v.z);
+    u.w[4 * i + 3] = __builtin_amdgcn_readfirstlane(v.w);
+  }
+  return u.r;
+}
+
+// The chunks of one workgroup, every gridDim.x-th one (the grid has no more workgroups than chunks).  From the last chunk down
+// when `down`: the pass that reads the gradients a second time starts with what the first one read last, which the 256 MB
+// last-level cache may still hold.  before() runs with the first record on its way.
+template <typename B, typename F>
+__device__ __forceinline__ void for_chunks(const ListView& l, bool down, B&& before, F&& fn) {
+  long long c = blockIdx.x;
+  auto record = [&](long long k) { return record_of(l.chunks + (down ? l.n_chunks - 1 - k : k)); };
+  ChunkRec r = record(c);
+  before();
+  while (true) {
+    fn(r);
+    c += gridDim.x;
+    if (c >= l.n_chunks) return;
+    r = record(c);
+  }
+}
+
+// First pass.  HBM-bound: one read of the gradients (and of the parameters with l2).  Squares are summed in 64 bits: fp32
+// squares of a gradient of 1e-25 vanish and those of 1e25 overflow; the conversion and the 64-bit fma run at rates that
+// leave the memory the bound.
 __global__ void __launch_bounds__(kTThreads) tensors_sumsq_kernel(ListView l, const float* denom, float scale_const, float l2) {
   __shared__ double red[kTThreads / 64];
   const float sc = scale_of(denom, scale_const);
   double acc = 0.0;
-  for (long long c = blockIdx.x; c < l.n_chunks; c += gridDim.x) {
-    const uint2 m = l.map[c];
-    const TensorRec& r = l.recs[m.x];
-    const long long first = (long long)m.y * kChunk, last = min(first + kChunk, r.n);
-    for (long long i = first + threadIdx.x; i < last; i += kTThreads) {
-      float e = load_elem(r.grad, r.grad_dtype, i) * sc;
-      if (l2 != 0.f) e = fmaf(l2, r.param[i], e);
-      acc += (double)e * (double)e;
-    }
-  }
+  for_chunks(l, false, [] {}, [&](const ChunkRec& r) {
+    with_type(r.grad_dtype, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      const T* g = static_cast<const T*>(r.grad);
+      walk_chunk<16 / sizeof(T)>(r.n, [&](auto at, auto ok, auto pieces, auto width) {
+        constexpr int K = decltype(pieces)::value, V = decltype(width)::value;
+        float e[K][V];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (ok(k)) load_piece<V>(g + at(k), e[k]);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!ok(k)) continue;
+          float p[V] = {};
+          if (l2 != 0.f) load_piece<V>(r.param + at(k), p);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float v = fmaf(l2, p[j], e[k][j] * sc);
+            acc += (double)v * (double)v;
+          }
+        }
+      });
+    });
+  });
   acc = block_sum_f64(acc, red);
   if (threadIdx.x == 0) l.partials[blockIdx.x] = acc;
 }
@@ -130,47 +198,90 @@ __global__ void __launch_bounds__(kTThreads) tensors_clip_kernel(ListView l, int
                                                                  float scale_const, float clip_norm, float* out_norm) {
   __shared__ double red[kTThreads / 64];
   const float sc = scale_of(denom, scale_const);
-  float norm;
-  const float f = clip_factor(partials_sum(l.partials, n_partials, red), clip_norm, &norm);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && out_norm) out_norm[0] = norm;
-  for (long long c = blockIdx.x; c < l.n_chunks; c += gridDim.x) {
-    const uint2 m = l.map[c];
-    const TensorRec& r = l.recs[m.x];
-    const long long first = (long long)m.y * kChunk, last = min(first + kChunk, r.n);
-    for (long long i = first + threadIdx.x; i < last; i += kTThreads)
-      store_elem(r.out, r.grad_dtype, i, load_elem(r.grad, r.grad_dtype, i) * sc * f);
-  }
+  float f = 1.f;
+  auto factor = [&] {
+    float norm;
+    f = clip_factor(partials_sum(l.partials, n_partials, red), clip_norm, &norm);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && out_norm) out_norm[0] = norm;
+  };
+  for_chunks(l, true, factor, [&](const ChunkRec& r) {
+    with_type(r.grad_dtype, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      const T* g = static_cast<const T*>(r.grad);
+      T* o = static_cast<T*>(r.out);
+      walk_chunk<16 / sizeof(T)>(r.n, [&](auto at, auto ok, auto pieces, auto width) {
+        constexpr int K = decltype(pieces)::value, V = decltype(width)::value;
+        float e[K][V];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (ok(k)) load_piece<V>(g + at(k), e[k]);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!ok(k)) continue;
+#pragma unroll
+          for (int j = 0; j < V; ++j) e[k][j] = e[k][j] * sc * f;
+          store_piece<V>(o + at(k), e[k]);
+        }
+      });
+    });
+  });
 }
 
+// Second pass of the update.  HBM-bound: reads gradient, parameter and accumulator, writes the last two and the copy.
 __global__ void __launch_bounds__(kTThreads) tensors_update_kernel(ListView l, int n_partials, const float* denom,
                                                                    float scale_const, float l2, float clip_norm, float lr,
                                                                    int strategy, float* out_norm) {
   __shared__ double red[kTThreads / 64];
   const float sc = scale_of(denom, scale_const);
   float f = 1.f;
-  if (n_partials > 0) {
+  auto factor = [&] {
+    if (n_partials == 0) return;
     float norm;
     f = clip_factor(partials_sum(l.partials, n_partials, red), clip_norm, &norm);
     if (blockIdx.x == 0 && threadIdx.x == 0 && out_norm) out_norm[0] = norm;
-  }
-  for (long long c = blockIdx.x; c < l.n_chunks; c += gridDim.x) {
-    const uint2 m = l.map[c];
-    const TensorRec& r = l.recs[m.x];
-    const long long first = (long long)m.y * kChunk, last = min(first + kChunk, r.n);
-    for (long long i = first + threadIdx.x; i < last; i += kTThreads) {
-      float t = r.param[i];
-      const float e = fmaf(l2, t, load_elem(r.grad, r.grad_dtype, i) * sc) * f;
-      if (strategy == ULTR_OPT_ADAGRAD) {
-        const float a = fmaf(e, e, r.accum[i]);
-        r.accum[i] = a;
-        t -= lr * e / sqrtf(a);
-      } else {
-        t -= lr * e;
-      }
-      r.param[i] = t;
-      if (r.copy) store_elem(r.copy, r.copy_dtype, i, t);
-    }
-  }
+  };
+  const bool ada = strategy == ULTR_OPT_ADAGRAD;
+  for_chunks(l, true, factor, [&](const ChunkRec& r) {
+    with_type(r.grad_dtype, [&](auto* gt) {
+      using T = std::remove_pointer_t<decltype(gt)>;
+      const T* g = static_cast<const T*>(r.grad);
+      walk_chunk<4>(r.n, [&](auto at, auto ok, auto pieces, auto width) {
+        constexpr int K = decltype(pieces)::value, V = decltype(width)::value;
+        float e[K][V], t[K][V], a[K][V];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!ok(k)) continue;
+          load_piece<V>(g + at(k), e[k]);
+          load_piece<V>(r.param + at(k), t[k]);
+          if (ada) load_piece<V>(r.accum + at(k), a[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          if (!ok(k)) continue;
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const float v = fmaf(l2, t[k][j], e[k][j] * sc) * f;
+            if (ada) {
+              a[k][j] = fmaf(v, v, a[k][j]);
+              t[k][j] -= lr * v / sqrtf(a[k][j]);
+            } else {
+              t[k][j] -= lr * v;
+            }
+          }
+          store_piece<V>(r.param + at(k), t[k]);
+          if (ada) store_piece<V>(r.accum + at(k), a[k]);
+        }
+        if (r.copy) {
+          with_type(r.copy_dtype, [&](auto* ct) {
+            using C = std::remove_pointer_t<decltype(ct)>;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+              if (ok(k)) store_piece<V>(static_cast<C*>(r.copy) + at(k), t[k]);
+          });
+        }
+      });
+    });
+  });
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -237,9 +348,8 @@ static int check_plan(const char* who, const UltrTensorPlan* p, int need) {
   return ULTR_OK;
 }
 static ListView view_of(const UltrTensorPlan* p) {
-  const TableLayout t = table_layout(p->n_tensors, p->n_chunks);
   char* b = static_cast<char*>(p->table);
-  return ListView{reinterpret_cast<TensorRec*>(b), reinterpret_cast<uint2*>(b + t.map), reinterpret_cast<double*>(b + t.partials), p->n_chunks};
+  return ListView{reinterpret_cast<double*>(b), reinterpret_cast<const ChunkRec*>(b + kPartialBytes), p->n_chunks};
 }
 static int pass_blocks(long long n_chunks) { return (int)std::min<long long>(n_chunks, kTMaxBlocks); }
 
@@ -269,7 +379,7 @@ using namespace ultr;
 extern "C" long long ultr_tensors_table_bytes(const UltrTensor* tensors_h, int n_tensors) {
   long long chunks = 0;
   if (check_list("ultr_tensors_table_bytes", tensors_h, n_tensors, &chunks) != ULTR_OK) return -1;
-  return table_layout(n_tensors, chunks).bytes;
+  return table_bytes_of(chunks);
 }
 
 extern "C" int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, void* table, long long table_bytes,
@@ -280,8 +390,8 @@ extern "C" int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, voi
   long long chunks = 0;
   int rc = check_list(who, tensors_h, n_tensors, &chunks);
   if (rc) return rc;
-  const TableLayout lay = table_layout(n_tensors, chunks);
-  ULTR_REQUIRE(table_bytes >= lay.bytes, ULTR_EINVAL, "%s: table of %lld bytes, %lld needed", who, table_bytes, lay.bytes);
+  ULTR_REQUIRE(table_bytes >= table_bytes_of(chunks), ULTR_EINVAL, "%s: table of %lld bytes, %lld needed", who, table_bytes,
+               table_bytes_of(chunks));
   try {
     rc = check_overlap(who, tensors_h, n_tensors);
   } catch (const std::bad_alloc&) {
@@ -290,27 +400,25 @@ extern "C" int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, voi
   }
   if (rc) return rc;
   int has = 7;
-  char* base = static_cast<char*>(table);
+  ChunkRec* recs = reinterpret_cast<ChunkRec*>(static_cast<char*>(table) + kPartialBytes);
   long long chunk = 0;
   for (int t0 = 0; t0 < n_tensors; t0 += kFillTensors) {
     FillArgs a{};
-    a.first_tensor = t0;
-    a.count = std::min(kFillTensors, n_tensors - t0);
-    long long most = 1;
-    for (int k = 0; k < a.count; ++k) {
-      const UltrTensor& u = tensors_h[t0 + k];
-      a.rec[k] = TensorRec{u.grad, u.out, u.param, u.accum, u.copy, u.n, u.grad_dtype, u.copy_dtype};
+    const int count = std::min(kFillTensors, n_tensors - t0);
+    long long most = 0;
+    for (int k = 0; k < count; ++k) {
+      const UltrTensor& u = a.t[k] = tensors_h[t0 + k];
       a.first_chunk[k] = chunk;
-      const long long c = (u.n + kChunk - 1) / kChunk;
+      const long long c = cdiv(u.n, kChunk);
       chunk += c;
       most = std::max(most, c);
       if (u.n > 0) has &= (u.out ? 1 : 0) | (u.param ? 2 : 0) | (u.accum ? 4 : 0);
     }
-    const int gy = (int)std::min<long long>(cdiv(most, kTThreads), 64);
+    if (most == 0) continue;
     {
       ProfScope prof_("tensors_fill_kernel", as_stream(stream));
-      hipLaunchKernelGGL(tensors_fill_kernel, dim3(a.count, gy), dim3(kTThreads), 0, as_stream(stream), a,
-                         reinterpret_cast<TensorRec*>(base), reinterpret_cast<uint2*>(base + lay.map));
+      hipLaunchKernelGGL(tensors_fill_kernel, dim3(count, (unsigned)std::min<long long>(cdiv(most, kTThreads), 64)), dim3(kTThreads),
+                         0, as_stream(stream), a, recs);
     }
     rc = check_launch("tensors_fill_kernel");
     if (rc) return rc;
