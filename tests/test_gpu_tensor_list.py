@@ -320,3 +320,26 @@ def test_a_ranker_of_ones_own_trains():
         assert abs(float(got) - norm) <= 1e-5 * norm
         for p, (rp, _, _, _) in zip(params, ref):
             assert (p.double() - rp).abs().max() <= 1e-5 * lr / 0.1 ** 0.5 + 2 * U
+
+
+def test_lists_larger_than_the_last_level_cache():
+    """Beyond 64 M elements the passes send data past the caches: same results."""
+    from ultra_amd.learning_algorithm import GradientTensors
+    sizes = [70000003, 5, 4097, 0, 8195]
+    grads, params = tensors(sizes, (BF16, F32), 1, aligned=False), tensors(sizes, (F32,), 2, aligned=False)
+    accums = [t.abs().add_(0.1) for t in tensors(sizes, (F32,), 3)]
+    copies = tensors(sizes, (F16, BF16), 4, aligned=False)
+    norm, ref = ref_update(grads, params, accums, 0.5, 0.01, 3.0, 0.05, True)
+    plan = GradientTensors(grads, out=[torch.empty_like(g) for g in grads], params=params, accums=accums, copies=copies)
+    out, plain = plan.clip(3.0, scale=0.5)
+    want = 0.5 * ref_norm(grads)
+    assert abs(float(plain) - want) <= 4 * U * want
+    for o, g in zip(out, grads):
+        w = g.double() * 0.5 * (3.0 / want)
+        within(o, w, 5 * U * w.abs() + half_step(g.dtype, w), 'out')
+    got = plan.clip_adagrad(3.0, 0.05, scale=0.5, l2=0.01)
+    assert abs(float(got) - norm) <= 8 * U * norm
+    for p, a, c, (rp, tp, ra, ta) in zip(params, accums, copies, ref):
+        within(p, rp, tp, 'param')
+        within(a, ra, ta, 'accum')
+        assert torch.equal(c, p.to(c.dtype))

@@ -19,18 +19,22 @@ template <typename T, int V>
 struct Piece {
   typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
 };
-template <int V, typename T>
+// NT: past the caches, for data that nothing reads again before it would be gone from them anyway.
+template <int V, bool NT = false, typename T>
 __device__ __forceinline__ void load_piece(const T* p, float (&v)[V]) {
-  const auto q = *reinterpret_cast<const typename Piece<T, V>::type*>(p);
+  typedef const typename Piece<T, V>::type P;
+  const auto q = NT ? __builtin_nontemporal_load(reinterpret_cast<P*>(p)) : *reinterpret_cast<P*>(p);
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] = to_f32(q[j]);
 }
-template <int V, typename T>
+template <int V, bool NT = false, typename T>
 __device__ __forceinline__ void store_piece(T* p, const float (&v)[V]) {
-  typename Piece<T, V>::type q;
+  typedef typename Piece<T, V>::type P;
+  P q;
 #pragma unroll
   for (int j = 0; j < V; ++j) q[j] = from_f32<T>(v[j]);
-  *reinterpret_cast<typename Piece<T, V>::type*>(p) = q;
+  if (NT) __builtin_nontemporal_store(q, reinterpret_cast<P*>(p));
+  else *reinterpret_cast<P*>(p) = q;
 }
 
 static inline bool known_dtype(int d) { return d == ULTR_DTYPE_F32 || d == ULTR_DTYPE_BF16 || d == ULTR_DTYPE_F16; }
