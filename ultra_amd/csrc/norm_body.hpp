@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 // of d_gamma and d_beta in registers over the whole walk.  What the row groups of a workgroup hold meets in LDS at the end
 // and leaves as one partial row (or the result itself when there is one workgroup).  16 elements a thread and 512 threads:
 // 16384 rows of 4096 bf16 77 us = 5.2 TB/s; with 1024 threads the registers spill (102 us), without the prefetch 8192 rows
-// of 8192 take 100 us against 81.
+// of 8192 take 100 us against 81.  Nothing needs x and dy after this, so they do not stay in the caches (40960 rows of 512
+// fp32: 45 us, 50 with plain loads) -- but for odd widths, whose pieces share cache lines with their neighbours.
 template <typename T, typename W, int TPR, int C, int V, bool TAIL>
 __global__ void __launch_bounds__(kGradThreads)
     layer_norm_grad_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,
@@ -171,8 +172,9 @@ __global__ void __launch_bounds__(kGradThreads)
 #pragma unroll
     for (int c = 0; c < C; ++c)
       if (pc.any(c)) {
-        nx[c] = *reinterpret_cast<const PT*>(x + r * ldx + pc.at[c]);
-        nd[c] = *reinterpret_cast<const PT*>(dy + r * lddy + pc.at[c]);
+        const PT *px = reinterpret_cast<const PT*>(x + r * ldx + pc.at[c]), *pd = reinterpret_cast<const PT*>(dy + r * lddy + pc.at[c]);
+        nx[c] = TAIL ? *px : __builtin_nontemporal_load(px);
+        nd[c] = TAIL ? *pd : __builtin_nontemporal_load(pd);
       }
   };
   fetch(row);

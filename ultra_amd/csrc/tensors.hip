@@ -14,7 +14,7 @@ namespace ultr {
 
 constexpr int kTThreads = 256;
 constexpr int kChunk = 4096;       // elements of one tensor that one workgroup takes at a time
-constexpr int kTMaxBlocks = 2048;  // workgroups of a pass, and partial sums of a norm
+constexpr int kTMaxBlocks = 1536;  // workgroups of a pass, and partial sums of a norm
 // Lists of more chunks than this (64 M elements: their second pass moves 256 MB or more) do not fit the 256 MB last-level
 // cache: what will not be read again goes past the caches (NT), so that the last gradients of the first pass are still there
 // when the second one begins with them.  Clip of 553 M bf16: 542 us, 625 without; update of 151 M: 564 us, 666 without.
