@@ -254,3 +254,8 @@ def current_stream():
     if _raw_stream:
         return ctypes.c_void_p(_raw_stream(torch.cuda.current_device()))
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def stream_of(device):
+    """``current_stream`` of the device with this index, which the caller knows to be the current one."""
+    return _raw_stream(device) if _raw_stream else current_stream()
