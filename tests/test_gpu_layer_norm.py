@@ -202,7 +202,10 @@ def test_no_rows():
 
 
 @pytest.mark.parametrize('m,n', SIZES + [(257, 1), (300, 17), (70, 136), (4097, 10), (1000, 512), (70001, 3), (2050, 136), (513, 1500),
-                                         (130, 4096), (600, 5003)])
+                                         (130, 4096), (600, 5003),
+                                         # on both sides of where the pass changes: 512 and 1024 rows, 8192 and 32768 entries
+                                         (512, 1100), (513, 1100), (512, 8192), (513, 8192), (700, 8193), (1024, 8200), (1025, 8200),
+                                         (1030, 9001), (2100, 9000), (40, 32768), (40, 33001), (600, 33001)])
 def test_backward(m, n):
     from ultra_amd.ranking_model import layer_norm, layer_norm_backward
     for k, (t, w) in enumerate(TYPES):

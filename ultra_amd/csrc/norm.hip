@@ -36,35 +36,38 @@ static void forward_shape(int N, F&& fn) {
                 Shape<1024, 8, 8>{});
   }
 }
-// Backward: 16 elements a thread, up to the 512 threads of a workgroup.
+// Backward: 16 elements a thread, up to the 512 threads of a workgroup; rows that are only held for a moment (FEW) take more.
 constexpr int kGradWidth = 16 * kGradThreads;
-template <typename T, typename F>
+constexpr int kFewWidth32 = 32768;  // 16-bit types: every width
+template <typename T, bool FEW, typename F>
 static void grad_shape(int N, F&& fn) {
   if constexpr (sizeof(T) == 4) {
     if (N < 4) return fn(Shape<4, 1, 1>{});
+    if constexpr (FEW)
+      if (N > kGradWidth) return first_shape(N, fn, Shape<512, 8, 4>{}, Shape<1024, 8, 4>{});
     first_shape(N, fn, Shape<4, 1, 4>{}, Shape<4, 4, 4>{}, Shape<8, 4, 4>{}, Shape<16, 4, 4>{}, Shape<32, 4, 4>{}, Shape<64, 4, 4>{},
                 Shape<128, 4, 4>{}, Shape<256, 4, 4>{}, Shape<512, 4, 4>{});
   } else {
     if (N < 8) return fn(Shape<8, 1, 1>{});
+    if constexpr (FEW)
+      if (N > kGradWidth) return first_shape(N, fn, Shape<512, 4, 8>{}, Shape<1024, 4, 8>{}, Shape<1024, 8, 8>{});
     first_shape(N, fn, Shape<4, 1, 8>{}, Shape<4, 2, 8>{}, Shape<8, 2, 8>{}, Shape<16, 2, 8>{}, Shape<32, 2, 8>{}, Shape<64, 2, 8>{},
                 Shape<128, 2, 8>{}, Shape<256, 2, 8>{}, Shape<512, 2, 8>{});
   }
 }
 
-// Workgroups of the backward pass that holds rows = partial rows of d_gamma and d_beta, for row groups of `rg` rows.  One per
-// CU; half of them while each would get fewer than 3 turns (the partial rows cost more than the idle CUs: 1000 rows of 4096
-// bf16 14.3 us with 128, 15.4 with 256; 3000 rows 25.4 and 22.1).  Up to 4 turns one workgroup does it all: no second launch.
-static int grad_blocks(long long M, int rg) {
-  const long long turns = cdiv(M, rg);
-  if (turns <= 4) return 1;
-  return (int)std::min<long long>(turns, turns < 3 * 256 ? 128 : 256);
+// Which of the three backward passes: few rows in one launch; rows that a workgroup holds; wider ones.
+enum GradPass { kFew, kHeld, kWide };
+static GradPass grad_pass(long long M, int N, int x_dtype) {
+  if (N <= kGradWidth) return M <= 512 ? kFew : kHeld;
+  return M <= 1024 && (x_dtype != ULTR_DTYPE_F32 || N <= kFewWidth32) ? kFew : kWide;
 }
-static int grad_row_groups(int N, int x_dtype) {
-  int rg = 1;
-  auto set = [&](auto s) { rg = kGradThreads / decltype(s)::TPR; };
-  if (x_dtype == ULTR_DTYPE_F32) grad_shape<float>(N, set);
-  else grad_shape<bf16_t>(N, set);
-  return rg;
+// Row groups' workgroups of the held pass = its partial rows.  One per CU; half of them while each would get fewer than 3
+// turns (the partial rows cost more than the idle CUs: 1000 rows of 4096 bf16 14.3 us with 128, 15.4 with 256; 3000 rows
+// 25.4 and 22.1).
+static int held_blocks(long long M, int rg) {
+  const long long turns = cdiv(M, rg);
+  return (int)std::min<long long>(turns, turns < 3 * 256 ? 128 : 256);
 }
 // Row slices of the wide pass: about 512 workgroups, at least 4 rows each; a multiple of 8 (see the kernel) unless that few.
 static int wide_slices(long long M, int N, int x_dtype) {
@@ -72,8 +75,20 @@ static int wide_slices(long long M, int N, int x_dtype) {
   const long long s = std::min<long long>((512 / tiles + 7) / 8 * 8, M / 4);
   return (int)(s < 8 ? std::max<long long>(s, 1) : s / 8 * 8);
 }
+// Column threads of a workgroup in the few-rows pass: 8 of them (128 bytes of a row), more for wide rows so that about 128
+// workgroups sum columns (512 rows of 32768 fp32: 56 us with 128, 67 with 512).
+static int few_across(int N, int threads, int V) {
+  int a = 8;
+  while (N > kGradWidth && a < threads && (long long)a * a * 2 * 128 * 128 < ((long long)N / V) * (N / V)) a *= 2;
+  return a;
+}
 static int partial_rows(long long M, int N, int x_dtype) {
-  return N <= kGradWidth ? grad_blocks(M, grad_row_groups(N, x_dtype)) : wide_slices(M, N, x_dtype);
+  const GradPass p = grad_pass(M, N, x_dtype);
+  if (p == kWide) return wide_slices(M, N, x_dtype);
+  int parts = 0;
+  auto set = [&](auto s) { parts = held_blocks(M, kGradThreads / decltype(s)::TPR); };
+  if (p == kHeld) x_dtype == ULTR_DTYPE_F32 ? grad_shape<float, false>(N, set) : grad_shape<bf16_t, false>(N, set);
+  return parts;
 }
 
 // One grid holds fewer than 2^32 threads: longer matrices go in slabs of whole workgroups.
@@ -177,13 +192,19 @@ extern "C" int ultr_layer_norm_forward(const void* x, long long ldx, const void*
   return check_launch("layer_norm_kernel");
 }
 
-// Partial rows of d_gamma and d_beta, behind the row sums of the wide pass.  The types share one size: the larger.
-static long long sums_bytes(long long M, int N) { return N <= kGradWidth ? 0 : (M * 8 + 15) / 16 * 16; }
+// Row sums of the wide pass | partial rows of d_gamma and d_beta.
+static long long sums_bytes(long long M, int N, int x_dtype) {
+  return grad_pass(M, N, x_dtype) == kWide ? (M * 8 + 15) / 16 * 16 : 0;
+}
 extern "C" long long ultr_layer_norm_workspace_bytes(long long M, int N) {
   if (check_norm("ultr_layer_norm_workspace_bytes", M, N, ULTR_DTYPE_F32, ULTR_DTYPE_F32) != ULTR_OK) return -1;
   if (M == 0) return 0;
-  const long long p = std::max(partial_rows(M, N, ULTR_DTYPE_F32), partial_rows(M, N, ULTR_DTYPE_BF16));
-  return sums_bytes(M, N) + (p > 1 ? p * 2 * N * (long long)sizeof(float) : 0);
+  long long most = 0;  // the types share one size
+  for (int d : {ULTR_DTYPE_F32, ULTR_DTYPE_BF16}) {
+    const long long p = partial_rows(M, N, d);
+    most = std::max(most, sums_bytes(M, N, d) + (p > 1 ? p * 2 * N * (long long)sizeof(float) : 0));
+  }
+  return most;
 }
 
 extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const void* x, long long ldx, const float* stats,
@@ -211,17 +232,33 @@ extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const vo
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
     if (M == 0) return launch_dw_sum(nullptr, 0, N, (W*)d_gamma, (W*)d_beta, s);
+    const GradPass pass = grad_pass(M, N, x_dtype);
     const int parts = partial_rows(M, N, x_dtype);
-    float* part = dw && parts > 1 ? (float*)((char*)ws + sums_bytes(M, N)) : nullptr;
-    W *dg = part ? nullptr : (W*)d_gamma, *db = part ? nullptr : (W*)d_beta;
-    if (N <= kGradWidth) {
-      grad_shape<T>(N, [&](auto shape) {
+    float* part = dw && parts > 1 ? (float*)((char*)ws + sums_bytes(M, N, x_dtype)) : nullptr;
+    if (pass == kFew) {
+      grad_shape<T, true>(N, [&](auto shape) {
+        using S = decltype(shape);
+        constexpr int NT = S::TPR < kGradThreads ? kGradThreads : S::TPR, RG = NT / S::TPR;
+        int rt = NT / few_across(N, NT, S::V);
+        while (rt > 1 && rt / 2 >= M) rt /= 2;
+        const int cols = dw ? (int)cdiv(N, NT / rt * S::V) : 0, rows = dx ? (int)cdiv(M, RG) : 0;
+        auto go = [&](auto tail) {
+          ProfScope prof_("layer_norm_grad_few_kernel", s);
+          hipLaunchKernelGGL((layer_norm_grad_few_kernel<T, W, S::TPR, S::C, S::V, decltype(tail)::value>), dim3(cols + rows),
+                             dim3(NT), 0, s, cols, rt, (const T*)dy, lddy, (const T*)x, ldx, stats, (const W*)gamma, (int)M, N,
+                             inv_n, (T*)dx, lddx, (W*)d_gamma, (W*)d_beta);
+        };
+        if (S::V > 1 && N % S::V) go(std::integral_constant<bool, (S::V > 1)>{});
+        else go(std::false_type{});
+      });
+    } else if (pass == kHeld) {
+      grad_shape<T, false>(N, [&](auto shape) {
         using S = decltype(shape);
         auto go = [&](auto tail) {
           ProfScope prof_("layer_norm_grad_kernel", s);
           hipLaunchKernelGGL((layer_norm_grad_kernel<T, W, S::TPR, S::C, S::V, decltype(tail)::value>), dim3(parts),
                              dim3(kGradThreads), 0, s, (const T*)dy, lddy, (const T*)x, ldx, stats, (const W*)gamma, M, N, inv_n,
-                             (T*)dx, lddx, part, dg, db);
+                             (T*)dx, lddx, part);
         };
         if (S::V > 1 && N % S::V) go(std::integral_constant<bool, (S::V > 1)>{});
         else go(std::false_type{});
@@ -231,21 +268,22 @@ extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const vo
       float2* sums = (float2*)ws;
       auto go = [&](auto tail) {
         constexpr bool TAIL = decltype(tail)::value;
-        if (dx) {
+        auto row_sums_of = [&](auto threads) {
+          constexpr int NT = decltype(threads)::value;
           ProfScope prof_("layer_norm_row_sums_kernel", s);
-          // few rows: all the threads a workgroup can have; many: more rows at a time (4096 of 16384 bf16: 60 and 50 us)
-          const unsigned grid = (unsigned)std::min<long long>(M, 2048);
-          if (M >= 512)
-            hipLaunchKernelGGL((layer_norm_row_sums_kernel<T, W, V, TAIL, 256>), dim3(grid), dim3(256), 0, s, (const T*)dy, lddy,
-                               (const T*)x, ldx, stats, (const W*)gamma, M, N, inv_n, sums);
-          else
-            hipLaunchKernelGGL((layer_norm_row_sums_kernel<T, W, V, TAIL, 1024>), dim3(grid), dim3(1024), 0, s, (const T*)dy, lddy,
-                               (const T*)x, ldx, stats, (const W*)gamma, M, N, inv_n, sums);
+          hipLaunchKernelGGL((layer_norm_row_sums_kernel<T, W, V, TAIL, NT>), dim3((unsigned)std::min<long long>(M, 2048)), dim3(NT),
+                             0, s, (const T*)dy, lddy, (const T*)x, ldx, stats, (const W*)gamma, M, N, inv_n, sums);
+        };
+        // many rows: small workgroups, more rows at a time (4096 rows of 16384 bf16: 50 us, 60 with 1024 threads); the few
+        // that come here, fp32 beyond the width of the few-rows pass, take all the threads a workgroup can have
+        if (dx) {
+          if (sizeof(T) == 2 || M > 512) row_sums_of(std::integral_constant<int, 256>{});
+          else row_sums_of(std::integral_constant<int, sizeof(T) == 2 ? 256 : 1024>{});
         }
         ProfScope prof_("layer_norm_wide_grad_kernel", s);
         hipLaunchKernelGGL((layer_norm_wide_grad_kernel<T, W, V, TAIL>), dim3(parts, (unsigned)cdiv(N, kNThreads * V)),
                            dim3(kNThreads), 0, s, (const T*)dy, lddy, (const T*)x, ldx, stats, (const W*)gamma, sums, M, N, (T*)dx,
-                           lddx, part, dg, db);
+                           lddx, part, part ? nullptr : (W*)d_gamma, part ? nullptr : (W*)d_beta);
       };
       if (N % V) go(std::true_type{});
       else go(std::false_type{});

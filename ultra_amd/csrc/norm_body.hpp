@@ -137,21 +137,20 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 // Backward, rows that a workgroup holds.  HBM-bound: two reads and one write of the matrix.  A workgroup walks over the rows,
 // kGradThreads / TPR at a time, with the next ones on their way while these are worked on; a thread keeps its columns' share
 // of d_gamma and d_beta in registers over the whole walk.  What the row groups of a workgroup hold meets in LDS at the end
-// and leaves as one partial row (or the result itself when there is one workgroup).  16 elements a thread and 512 threads:
+// and leaves as one partial row.  16 elements a thread and 512 threads:
 // 16384 rows of 4096 bf16 77 us = 5.2 TB/s; with 1024 threads the registers spill (102 us), without the prefetch 8192 rows
 // of 8192 take 100 us against 81.  Nothing needs x and dy after this, so they do not stay in the caches (40960 rows of 512
 // fp32: 45 us, 50 with plain loads) -- but for odd widths, whose pieces share cache lines with their neighbours.
 template <typename T, typename W, int TPR, int C, int V, bool TAIL>
 __global__ void __launch_bounds__(kGradThreads)
     layer_norm_grad_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,
-                           long long M, int N, float inv_n, T* dx, long long lddx, float* ws, W* d_gamma, W* d_beta) {
+                           long long M, int N, float inv_n, T* dx, long long lddx, float* ws) {
   constexpr int NT = kGradThreads, RG = NT / TPR;
   typedef typename Piece<T, V>::type PT;
   __shared__ float red[2][2 * NT / 64];
   __shared__ __align__(16) float cols[NT * C * V];
   const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const Pieces<TPR, C, V, TAIL> pc(lane, N);
-  const bool dw = ws || d_gamma || d_beta;
   float g_w[C][V], acc_g[C][V], acc_b[C][V];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(kGradThreads)
       }
     }
   }
-  if (!dw) return;
+  if (!ws) return;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
@@ -232,8 +231,7 @@ __global__ void __launch_bounds__(kGradThreads)
 #pragma unroll
       for (int j = 0; j < V; ++j) cols[group * (TPR * C * V) + (c * TPR + lane) * V + j] = which ? acc_b[c][j] : acc_g[c][j];
     __syncthreads();
-    W* out = which ? d_beta : d_gamma;
-    float* part = ws ? ws + ((long long)blockIdx.x * 2 + which) * N : nullptr;
+    float* part = ws + ((long long)blockIdx.x * 2 + which) * N;
     for (int i = threadIdx.x; i < TPR * C * V; i += NT) {
       const int piece = i / V * V, at = TAIL ? min(piece, N - V) : piece;
       const int col = at + i % V;
@@ -241,9 +239,129 @@ __global__ void __launch_bounds__(kGradThreads)
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < RG; ++k) sum += cols[k * (TPR * C * V) + i];
-      if (part) part[col] = sum;
-      else if (out) out[col] = from_f32<W>(sum);
+      part[col] = sum;
     }
+  }
+}
+
+// Backward of few rows, in one launch and without a workspace: d_gamma and d_beta need the statistics, not dx, so the last
+// workgroups of the grid form dx, whole rows in registers, while the first ones sum columns.  Everything is read twice,
+// mostly out of a cache the second time; the pass above writes and re-reads partial rows instead, and takes a second launch.
+// 100 rows of 4096 bf16: 5.5 us, 9.0 the other way; 512 rows: 9.7 and 11.8; 1000 rows: 13 and 14.6, and beyond it loses.
+//
+// Columns: the threads of a workgroup as `rt` row threads times NT / rt threads of V columns each (8 at least: 128 bytes).
+template <typename T, typename W, int V, bool TAIL, int NT>
+__device__ __forceinline__ void few_columns(int block, int rt, const T* dy, long long lddy, const T* x, long long ldx,
+                                            const float* stats, int M, int N, W* d_gamma, W* d_beta, float* lds) {
+  const int across = NT / rt, lane = threadIdx.x & (across - 1), rl = threadIdx.x / across;
+  const int i = (block * across + lane) * V, at = TAIL ? min(i, N - V) : i;
+  float acc[2 * V];
+#pragma unroll
+  for (int j = 0; j < 2 * V; ++j) acc[j] = 0.f;
+  if (i < N) {
+#pragma unroll 4
+    for (int m = rl; m < M; m += rt) {
+      const float2 st = *reinterpret_cast<const float2*>(stats + 2 * m);
+      float vx[V], vd[V];
+      load_piece<V>(x + m * ldx + at, vx);
+      load_piece<V>(dy + m * lddy + at, vd);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        acc[j] = fmaf(vd[j], (vx[j] - st.x) * st.y, acc[j]);
+        acc[V + j] += vd[j];
+      }
+    }
+  }
+  // row threads that share a wave, then the waves that share columns
+  for (int d = across; d < 64; d <<= 1) {
+#pragma unroll
+    for (int j = 0; j < 2 * V; ++j) acc[j] += __shfl_xor(acc[j], d);
+  }
+  const int per_wave = across < 64 ? across : 64;       // threads of a wave that hold different columns
+  const int waves = across < 64 ? NT / 64 : NT / across;  // waves that hold the same ones
+  if (waves > 1) {
+    const int first = across < 64 ? 0 : (threadIdx.x / 64) % (across / 64), mine = across < 64 ? threadIdx.x / 64 : rl;
+    const int slot = first * 64 + (threadIdx.x & 63);
+    if ((threadIdx.x & 63) < per_wave) {
+#pragma unroll
+      for (int j = 0; j < 2 * V; ++j) lds[(mine * 2 * V + j) * across + slot] = acc[j];
+    }
+    __syncthreads();
+    if (mine > 0 || (threadIdx.x & 63) >= per_wave) return;
+    for (int w = 1; w < waves; ++w) {
+#pragma unroll
+      for (int j = 0; j < 2 * V; ++j) acc[j] += lds[(w * 2 * V + j) * across + slot];
+    }
+  } else if ((threadIdx.x & 63) >= per_wave) {
+    return;
+  }
+  if (i >= N) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (TAIL && at + j < i) continue;  // the piece before holds it
+    if (d_gamma) d_gamma[at + j] = from_f32<W>(acc[j]);
+    if (d_beta) d_beta[at + j] = from_f32<W>(acc[V + j]);
+  }
+}
+
+template <typename T, typename W, int TPR, int C, int V, bool TAIL>
+__global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR)
+    layer_norm_grad_few_kernel(int col_blocks, int rt, const T* dy, long long lddy, const T* x, long long ldx, const float* stats,
+                               const W* gamma, int M, int N, float inv_n, T* dx, long long lddx, W* d_gamma, W* d_beta) {
+  constexpr int NT = TPR < kGradThreads ? kGradThreads : TPR, RG = NT / TPR;
+  typedef typename Piece<T, V>::type PT;
+  __shared__ float lds[NT * 2 * V];
+  if ((int)blockIdx.x < col_blocks)
+    return few_columns<T, W, V, TAIL, NT>(blockIdx.x, rt, dy, lddy, x, ldx, stats, M, N, d_gamma, d_beta, lds);
+  const int lane = threadIdx.x % TPR, row = ((int)blockIdx.x - col_blocks) * RG + threadIdx.x / TPR;
+  const Pieces<TPR, C, V, TAIL> pc(lane, N);
+  const bool live = row < M;
+  const long long r = live ? row : M - 1;
+  const float2 st = *reinterpret_cast<const float2*>(stats + 2 * r);
+  PT px[C], pd[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (!pc.any(c)) continue;
+    px[c] = *reinterpret_cast<const PT*>(x + r * ldx + pc.at[c]);
+    pd[c] = *reinterpret_cast<const PT*>(dy + r * lddy + pc.at[c]);
+  }
+  auto normed = [&](int c, float (&xh)[V], float (&gr)[V]) {
+    float g[V];
+    if (gamma) load_piece<V>(gamma + pc.at[c], g);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      xh[j] = (to_f32(px[c][j]) - st.x) * st.y;
+      gr[j] = to_f32(pd[c][j]);
+      if (gamma) gr[j] *= g[j];
+    }
+  };
+  // 512 threads have registers for what the sums were made of; 1024 form it again (777 rows of 12345 bf16: 24 us, 27)
+  constexpr bool KEEP = NT == kGradThreads;
+  float xh[KEEP ? C : 1][V], gr[KEEP ? C : 1][V], s[2] = {0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (!pc.any(c)) continue;
+    const int k = KEEP ? c : 0;
+    normed(c, xh[k], gr[k]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float gc = pc.counted(c, j, gr[k][j]);
+      s[0] += gc;
+      s[1] = fmaf(gc, xh[k][j], s[1]);
+    }
+  }
+  row_sums<TPR>(s, lds);
+  if (!live) return;
+  const float a = s[0] * inv_n, b = s[1] * inv_n;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    if (!pc.any(c)) continue;
+    const int k = KEEP ? c : 0;
+    if (!KEEP) normed(c, xh[k], gr[k]);
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = st.y * (gr[k][j] - fmaf(xh[k][j], b, a));
+    store_piece<V>(dx + r * lddx + pc.at[c], v);
   }
 }
 
