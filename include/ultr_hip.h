@@ -266,7 +266,8 @@ int ultr_layer_norm_forward(const void* x, long long ldx, const void* gamma, con
 /* Its gradient.  With xh = (x - mean) * rstd from the forward pass's stats and g = dy * gamma:
  *   dx = rstd * (g - mean_N(g) - xh * mean_N(g * xh)) ;  d_gamma = sum_m dy * xh ;  d_beta = sum_m dy
  * dy, dx as x above (lddy, lddx); d_gamma, d_beta: [N] of w_dtype, written, not added to (zeros when M = 0).
- * dx, d_gamma and d_beta may each be NULL (not wanted), not all of them.  dx must not overlap x or dy.
+ * dx, d_gamma and d_beta may each be NULL (not wanted), not all of them.  No output may overlap an input or another output
+ * (checked for dx against x and dy, and among gamma, d_gamma, d_beta).
  * The sums over rows are fp32 in an order that depends on (M, N, types) only: equal calls give equal bits.
  * ws: ultr_layer_norm_workspace_bytes(M, N) bytes, 16-byte aligned, contents irrelevant before and after the call; may
  * be NULL when that is 0, or for dx alone at N <= 8192.  Two calls in flight need a workspace each. */
@@ -595,7 +596,7 @@ int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, void* table, l
 int ultr_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float* out_norm, void* stream);
 
 /* out = f * scale * grad for every tensor, f = clip_norm / max(norm, clip_norm) with the norm above (also written to
- * out_norm if that is not NULL).  clip_norm <= 0: f = 1.  A norm that is not finite makes f NaN, and so every output
+ * out_norm if that is not NULL).  clip_norm <= 0: f = 1; NaN is refused.  A norm that is not finite makes f NaN, and so every output
  * NaN (tf.clip_by_global_norm).  Needs `out` in every tensor. */
 int ultr_clip_by_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float clip_norm,
                              float* out_norm, void* stream);

@@ -235,6 +235,27 @@ def test_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(got, plan.out + params + accums + [plan.norm]))
 
 
+def test_a_graph_outlives_the_list_it_was_captured_with():
+    from ultra_amd.learning_algorithm import GradientTensors
+    grads = tensors(SIZES['small'], (F32,), 1)
+    plan = GradientTensors(grads)
+    plan.global_norm()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.global_norm()
+    plan.clip(1.0)  # makes the outputs and lays the list out again
+    waste = [torch.full((1 << 16,), 255, dtype=torch.uint8, device='cuda') for _ in range(64)]
+    for k in range(3):
+        grads[0].mul_(2.0)
+        plan.norm.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ref_norm(grads)
+        assert abs(float(plan.norm) - want) <= 4 * U * want
+    del waste
+
+
 def test_two_lists_in_flight():
     from ultra_amd.learning_algorithm import GradientTensors
     lists = []

@@ -52,6 +52,7 @@ def backward(**kw):
     (dict(lddy=7), -1, 'apart'), (dict(lddx=7), -1, 'apart'), (dict(dx=P), -1, 'overlaps'), (dict(dx=2 * P), -1, 'overlaps'),
     (dict(dx=2 * P + 60), -1, 'overlaps'), (dict(stats=P + 4), -1, 'aligned'), (dict(xd=F16, wd=BF16), -1, 'w_dtype'),
     (dict(N=65537, ldx=1 << 17, lddy=1 << 17, lddx=1 << 17), -2, 'too large'), (dict(dg=5 * P + 2), -1, 'aligned'),
+    (dict(db=5 * P + 28), -1, 'overlaps'), (dict(gamma=5 * P), -1, 'overlaps'), (dict(gamma=6 * P + 4), -1, 'overlaps'),
 ])
 def test_backward_refuses(kw, rc, text):
     assert backward(**kw) == rc
@@ -113,10 +114,19 @@ def test_calls_refuse_what_the_list_lacks():
     assert lib.ultr_global_norm(None, None, 1.0, P, None) == -1
     assert lib.ultr_global_norm(p, None, 1.0, None, None) == -1
     assert lib.ultr_clip_by_global_norm(p, None, 1.0, 1.0, P, None) == -1 and 'lacks out' in last()
+    assert lib.ultr_clip_by_global_norm(p, None, 1.0, float('nan'), P, None) == -1 and 'not a number' in last()
     assert lib.ultr_clip_adagrad_tensors(p, None, 1.0, 0.0, 1.0, 0.1, _lib.OPT_ADAGRAD, P, None) == -1 and 'lacks param accum' in last()
     p.has = 2
     assert lib.ultr_clip_adagrad_tensors(p, None, 1.0, 0.0, 1.0, 0.1, _lib.OPT_ADAGRAD, P, None) == -1 and 'lacks accum' in last()
     assert lib.ultr_clip_adagrad_tensors(p, None, 1.0, 0.0, 1.0, 0.1, 9, P, None) == -1 and 'grad_strategy' in last()
+
+
+def test_the_python_record_is_the_abi_record():
+    from ultra_amd.learning_algorithm.gradient_tensors import _REC
+    assert _REC.itemsize == ctypes.sizeof(_lib.UltrTensor)
+    for name, _ in _lib.UltrTensor._fields_:
+        assert _REC.fields[name][1] == getattr(_lib.UltrTensor, name).offset
+        assert _REC.fields[name][0].itemsize == getattr(_lib.UltrTensor, name).size
 
 
 def test_a_scorer_refuses_half_precision_storage():

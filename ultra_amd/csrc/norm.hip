@@ -223,6 +223,12 @@ extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const vo
                ULTR_EINVAL, "%s: gamma, d_gamma, d_beta, stats or ws not aligned", who);
   ULTR_REQUIRE(!rows_overlap(dx, lddx, x, ldx, M, N, x_dtype) && !rows_overlap(dx, lddx, dy, lddy, M, N, x_dtype), ULTR_EINVAL,
                "%s: dx overlaps x or dy", who);
+  auto share = [&](const void* a, const void* b) {  // two weight vectors that overlap
+    const uintptr_t bytes = (uintptr_t)N * dtype_bytes(w_dtype), pa = (uintptr_t)a, pb = (uintptr_t)b;
+    return a && b && pa < pb + bytes && pb < pa + bytes;
+  };
+  ULTR_REQUIRE(!share(d_gamma, d_beta) && !share(gamma, d_gamma) && !share(gamma, d_beta), ULTR_EINVAL,
+               "%s: d_gamma overlaps d_beta, or one of them gamma", who);
   const bool dw = d_gamma || d_beta;
   ULTR_REQUIRE((!dw && N <= kGradWidth) || ws || ultr_layer_norm_workspace_bytes(M, N) == 0, ULTR_EINVAL,
                "%s: workspace required", who);
@@ -231,6 +237,7 @@ extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const vo
   return with_types(x_dtype, w_dtype, [&](auto* t, auto* w) {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
+    if (M == 0 && !dw) return ULTR_OK;
     if (M == 0) return launch_dw_sum(nullptr, 0, N, (W*)d_gamma, (W*)d_beta, s);
     const GradPass pass = grad_pass(M, N, x_dtype);
     const int parts = partial_rows(M, N, x_dtype);

@@ -357,7 +357,8 @@ static int check_overlap(const char* who, const UltrTensor* t, int n) {
   return ULTR_OK;
 }
 
-static int check_plan(const char* who, const UltrTensorPlan* p, int need) {
+static int check_plan(const char* who, const UltrTensorPlan* p, int need, float clip_norm) {
+  ULTR_REQUIRE(clip_norm == clip_norm, ULTR_EINVAL, "%s: clip_norm is not a number", who);
   ULTR_REQUIRE(p && p->table && p->n_chunks >= 0 && p->n_tensors >= 0, ULTR_EINVAL, "%s: bad plan", who);
   ULTR_REQUIRE((p->has & need) == need, ULTR_EINVAL, "%s: the list lacks%s%s%s", who, (need & ~p->has & 1) ? " out" : "",
                (need & ~p->has & 2) ? " param" : "", (need & ~p->has & 4) ? " accum" : "");
@@ -446,7 +447,7 @@ extern "C" int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, voi
 
 extern "C" int ultr_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float* out_norm,
                                 void* stream) {
-  int rc = check_plan("ultr_global_norm", plan_h, 0);
+  int rc = check_plan("ultr_global_norm", plan_h, 0, 0.f);
   if (rc) return rc;
   ULTR_REQUIRE(out_norm, ULTR_EINVAL, "ultr_global_norm: null out_norm");
   const ListView l = view_of(plan_h);
@@ -456,7 +457,7 @@ extern "C" int ultr_global_norm(const UltrTensorPlan* plan_h, const float* denom
 
 extern "C" int ultr_clip_by_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float clip_norm,
                                         float* out_norm, void* stream) {
-  int rc = check_plan("ultr_clip_by_global_norm", plan_h, 1);
+  int rc = check_plan("ultr_clip_by_global_norm", plan_h, 1, clip_norm);
   if (rc) return rc;
   const ListView l = view_of(plan_h);
   hipStream_t s = as_stream(stream);
@@ -474,7 +475,7 @@ extern "C" int ultr_clip_adagrad_tensors(const UltrTensorPlan* plan_h, const flo
                                          float clip_norm, float lr, int strategy, float* out_norm, void* stream) {
   const char* who = "ultr_clip_adagrad_tensors";
   ULTR_REQUIRE(strategy == ULTR_OPT_ADAGRAD || strategy == ULTR_OPT_SGD, ULTR_EINVAL, "%s: grad_strategy=%d", who, strategy);
-  int rc = check_plan(who, plan_h, strategy == ULTR_OPT_ADAGRAD ? 6 : 2);
+  int rc = check_plan(who, plan_h, strategy == ULTR_OPT_ADAGRAD ? 6 : 2, clip_norm);
   if (rc) return rc;
   const ListView l = view_of(plan_h);
   hipStream_t s = as_stream(stream);

@@ -6,11 +6,14 @@ ipw_rank.py:155-165).  The learning algorithms of this package keep their variab
 """
 import ctypes
 
+import numpy as np
 import torch
 
 from .. import _lib
 
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_REC = np.dtype([('grad', 'u8'), ('out', 'u8'), ('param', 'u8'), ('accum', 'u8'), ('copy', 'u8'), ('n', 'i8'),
+                 ('grad_dtype', 'i4'), ('copy_dtype', 'i4')])  # _lib.UltrTensor, filled a column at a time
 _STRATEGY = {'ada': _lib.OPT_ADAGRAD, 'sgd': _lib.OPT_SGD}  # the grad_strategy hparam
 
 
@@ -34,16 +37,19 @@ class GradientTensors(object):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('GradientTensors lays its list out on the device: build it before the capture')
         self.grads = list(grads)
-        self.device = torch.device('cuda', torch.cuda.current_device())
+        self._index = torch.cuda.current_device()
+        self.device = torch.device('cuda', self._index)
         self.params, self.accums, self.copies = (None if v is None else list(v) for v in (params, accums, copies))
         self.out = None if out is None else list(out)
-        for name, want in (('out', None), ('params', torch.float32), ('accums', torch.float32), ('copies', False)):
-            self._check_role(name, want)
         for k, g in enumerate(self.grads):
-            if g.dtype not in _DTYPE or g.device != self.device or not g.is_contiguous():
+            if g.dtype not in _DTYPE or g.get_device() != self._index or not g.is_contiguous():
                 raise ValueError('grads[%d]: a contiguous float32, bfloat16 or float16 tensor on %s expected, got %s on %s'
                                  % (k, self.device, g.dtype, g.device))
+        for name, want in (('out', None), ('params', torch.float32), ('accums', torch.float32), ('copies', False)):
+            self._check_role(name, want)
         self.norm = torch.zeros(1, dtype=torch.float32, device=self.device)
+        self._norm_ptr = self.norm.data_ptr()
+        self._tables = []
         self._build()
 
     def _check_role(self, name, dtype):
@@ -56,51 +62,52 @@ class GradientTensors(object):
             if t is None and dtype is False:
                 continue
             ok = t.dtype in _DTYPE if dtype is False else t.dtype == (g.dtype if dtype is None else dtype)
-            if not ok or t.shape != g.shape or t.device != self.device or not t.is_contiguous():
+            if not ok or t.shape != g.shape or t.get_device() != self._index or not t.is_contiguous():
                 raise ValueError('%s[%d]: contiguous %s %s on %s expected, got %s %s on %s'
                                  % (name, k, dtype or g.dtype, tuple(g.shape), self.device, t.dtype, tuple(t.shape), t.device))
 
     def _build(self):
         n = len(self.grads)
-        rec = (_lib.UltrTensor * max(n, 1))()
-        for k, g in enumerate(self.grads):
-            r = rec[k]
-            r.grad, r.n, r.grad_dtype = g.data_ptr(), g.numel(), _DTYPE[g.dtype]
-            if self.out is not None:
-                r.out = self.out[k].data_ptr()
-            if self.params is not None:
-                r.param = self.params[k].data_ptr()
-            if self.accums is not None:
-                r.accum = self.accums[k].data_ptr()
-            if self.copies is not None and self.copies[k] is not None:
-                r.copy, r.copy_dtype = self.copies[k].data_ptr(), _DTYPE[self.copies[k].dtype]
+        rec = np.zeros(n, dtype=_REC)
+        rec['grad'] = [g.data_ptr() for g in self.grads]
+        rec['n'] = [g.numel() for g in self.grads]
+        rec['grad_dtype'] = [_DTYPE[g.dtype] for g in self.grads]
+        for name, tensors in (('out', self.out), ('param', self.params), ('accum', self.accums)):
+            if tensors is not None:
+                rec[name] = [t.data_ptr() for t in tensors]
+        if self.copies is not None:
+            rec['copy'] = [0 if t is None else t.data_ptr() for t in self.copies]
+            rec['copy_dtype'] = [0 if t is None else _DTYPE[t.dtype] for t in self.copies]
         lib = _lib.lib()
-        nbytes = lib.ultr_tensors_table_bytes(rec, n)
+        ptr = rec.ctypes.data_as(ctypes.POINTER(_lib.UltrTensor))
+        nbytes = lib.ultr_tensors_table_bytes(ptr, n)
         if nbytes < 0:
             raise _lib.UltrError(lib.ultr_last_error().decode())
-        self._table = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        self._plan = _lib.UltrTensorPlan()
-        _lib.check(lib.ultr_tensors_plan(rec, n, _lib.ptr(self._table), nbytes, self._plan, _lib.current_stream()),
-                   'ultr_tensors_plan')
+        table = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        self._tables.append(table)  # an earlier one stays: a captured graph may read it
+        plan = _lib.UltrTensorPlan()
+        _lib.check(lib.ultr_tensors_plan(ptr, n, _lib.ptr(table), nbytes, plan, _lib.current_stream()), 'ultr_tensors_plan')
         # whichever stream uses the plan later finds it written
         torch.cuda.current_stream().synchronize()
+        self._plan = ctypes.pointer(plan)
 
     def _stream(self):
-        if torch.cuda.current_device() != self.device.index:
+        if torch.cuda.current_device() != self._index:
             raise ValueError('these tensors live on %s, the current device is cuda:%d' % (self.device, torch.cuda.current_device()))
-        return _lib.current_stream()
+        return _lib.stream_of(self._index)
 
     def _denom(self, denom):
         if denom is None:
             return None
-        if denom.device != self.device or denom.dtype != torch.float32 or denom.numel() < 1:
+        if denom.get_device() != self._index or denom.dtype != torch.float32 or denom.numel() < 1:
             raise ValueError('denom: a float32 device scalar expected')
         return denom.data_ptr()
 
     def global_norm(self, denom=None, scale=1.0):
         """sqrt of the sum over all gradients of (scale / denom * g)^2, a device tensor [1] that the next call overwrites."""
-        _lib.check(_lib.lib().ultr_global_norm(self._plan, self._denom(denom), scale, self.norm.data_ptr(), self._stream()),
-                   'ultr_global_norm')
+        rc = _lib._lib.ultr_global_norm(self._plan, self._denom(denom), scale, self._norm_ptr, self._stream())
+        if rc:
+            _lib.check(rc, 'ultr_global_norm')
         return self.norm
 
     def clip(self, clip_norm, denom=None, scale=1.0):
@@ -111,8 +118,9 @@ class GradientTensors(object):
                 raise RuntimeError('clip: give ``out`` to the constructor before capturing')
             self.out = [torch.empty_like(g) for g in self.grads]
             self._build()
-        _lib.check(_lib.lib().ultr_clip_by_global_norm(self._plan, self._denom(denom), scale, clip_norm,
-                                                       self.norm.data_ptr(), self._stream()), 'ultr_clip_by_global_norm')
+        rc = _lib._lib.ultr_clip_by_global_norm(self._plan, self._denom(denom), scale, clip_norm, self._norm_ptr, self._stream())
+        if rc:
+            _lib.check(rc, 'ultr_clip_by_global_norm')
         return self.out, self.norm
 
     def clip_adagrad(self, clip_norm, learning_rate, denom=None, scale=1.0, l2=0.0, grad_strategy='ada'):
@@ -124,7 +132,8 @@ class GradientTensors(object):
         strategy = _STRATEGY.get(grad_strategy)
         if strategy is None:
             raise ValueError("grad_strategy '%s' unknown (ada, sgd)" % grad_strategy)
-        _lib.check(_lib.lib().ultr_clip_adagrad_tensors(self._plan, self._denom(denom), scale, l2, clip_norm, learning_rate,
-                                                        strategy, self.norm.data_ptr(), self._stream()),
-                   'ultr_clip_adagrad_tensors')
+        rc = _lib._lib.ultr_clip_adagrad_tensors(self._plan, self._denom(denom), scale, l2, clip_norm, learning_rate, strategy,
+                                                 self._norm_ptr, self._stream())
+        if rc:
+            _lib.check(rc, 'ultr_clip_adagrad_tensors')
         return self.norm
