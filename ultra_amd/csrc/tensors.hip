@@ -67,15 +67,15 @@ __global__ void __launch_bounds__(kTThreads) tensors_fill_kernel(FillArgs a, Chu
   }
 }
 
-// Sum of one double per thread over the workgroup, fixed order; valid in every thread.
+// Sum of one double per thread over the workgroup, fixed order; valid in every thread.  Once per kernel (red is not reused).
 __device__ __forceinline__ double block_sum_f64(double v, double* red) {
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
+  lds_barrier();
   double s = 0.0;
-  for (int w = 0; w < (int)(blockDim.x >> 6); ++w) s += red[w];
+#pragma unroll
+  for (int w = 0; w < kTThreads / 64; ++w) s += red[w];
   return s;
 }
 
@@ -138,15 +138,14 @@ __device__ __forceinline__ ChunkRec record_of(const ChunkRec* p) {
 
 // The chunks of one workgroup, every gridDim.x-th one.  With `down` the last of them first: the pass that reads the gradients
 // a second time starts with what the first one read last, and an XCD (workgroups go to the 8 XCDs in turn) meets its own
-// chunks again.  before() runs with the first record on its way.
-template <typename B, typename F>
-__device__ __forceinline__ void for_chunks(const ChunkRec* chunks, long long n_chunks, bool down, B&& before, F&& fn) {
+// chunks again.
+template <typename F>
+__device__ __forceinline__ void for_chunks(const ChunkRec* chunks, long long n_chunks, bool down, F&& fn) {
   long long c = blockIdx.x;
   if (c >= n_chunks) return;
   const long long step = down ? -(long long)gridDim.x : (long long)gridDim.x;
   if (down) c += (n_chunks - 1 - c) / gridDim.x * gridDim.x;
   ChunkRec r = record_of(chunks + c);
-  before();
   while (true) {
     fn(r);
     c += step;
@@ -190,8 +189,8 @@ __global__ void __launch_bounds__(kTThreads) tensors_sumsq_kernel(ListView l, co
   double acc = 0.0;
   // whole turns of the grid, so that a chunk belongs to the same workgroup in both passes
   const long long past = STREAM ? max(l.n_chunks - kKeepChunks, 0ll) / gridDim.x * gridDim.x : 0;
-  if (STREAM) for_chunks(l.chunks, past, false, [] {}, [&](const ChunkRec& r) { add_squares<true>(r, sc, l2, acc); });
-  for_chunks(l.chunks + past, l.n_chunks - past, false, [] {}, [&](const ChunkRec& r) { add_squares<false>(r, sc, l2, acc); });
+  if (STREAM) for_chunks(l.chunks, past, false, [&](const ChunkRec& r) { add_squares<true>(r, sc, l2, acc); });
+  for_chunks(l.chunks + past, l.n_chunks - past, false, [&](const ChunkRec& r) { add_squares<false>(r, sc, l2, acc); });
   acc = block_sum_f64(acc, red);
   if (threadIdx.x == 0) l.partials[blockIdx.x] = acc;
 }
@@ -214,12 +213,15 @@ __global__ void __launch_bounds__(kTThreads) tensors_clip_kernel(ListView l, int
   __shared__ double red[kTThreads / 64];
   const float sc = scale_of(denom, scale_const);
   float f = 1.f;
-  auto factor = [&] {
+  bool pending = true;
+  auto factor = [&] {  // the norm, once, with the first chunk's elements on their way; every thread comes here
+    if (!pending) return;
+    pending = false;
     float norm;
     f = clip_factor(partials_sum(l.partials, n_partials, red), clip_norm, &norm);
     if (blockIdx.x == 0 && threadIdx.x == 0 && out_norm) out_norm[0] = norm;
   };
-  for_chunks(l.chunks, l.n_chunks, true, factor, [&](const ChunkRec& r) {
+  for_chunks(l.chunks, l.n_chunks, true, [&](const ChunkRec& r) {
     with_type(r.grad_dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       const T* g = static_cast<const T*>(r.grad);
@@ -230,6 +232,7 @@ __global__ void __launch_bounds__(kTThreads) tensors_clip_kernel(ListView l, int
 #pragma unroll
         for (int k = 0; k < K; ++k)
           if (ok(k)) load_piece<V, STREAM>(g + at(k), e[k]);
+        factor();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!ok(k)) continue;
@@ -250,14 +253,16 @@ __global__ void __launch_bounds__(kTThreads) tensors_update_kernel(ListView l, i
   __shared__ double red[kTThreads / 64];
   const float sc = scale_of(denom, scale_const);
   float f = 1.f;
-  auto factor = [&] {
-    if (n_partials == 0) return;
+  bool pending = n_partials > 0;
+  auto factor = [&] {  // as above
+    if (!pending) return;
+    pending = false;
     float norm;
     f = clip_factor(partials_sum(l.partials, n_partials, red), clip_norm, &norm);
     if (blockIdx.x == 0 && threadIdx.x == 0 && out_norm) out_norm[0] = norm;
   };
   const bool ada = strategy == ULTR_OPT_ADAGRAD;
-  for_chunks(l.chunks, l.n_chunks, true, factor, [&](const ChunkRec& r) {
+  for_chunks(l.chunks, l.n_chunks, true, [&](const ChunkRec& r) {
     with_type(r.grad_dtype, [&](auto* gt) {
       using T = std::remove_pointer_t<decltype(gt)>;
       const T* g = static_cast<const T*>(r.grad);
@@ -271,6 +276,7 @@ __global__ void __launch_bounds__(kTThreads) tensors_update_kernel(ListView l, i
           load_piece<V, STREAM>(r.param + at(k), t[k]);
           if (ada) load_piece<V, STREAM>(r.accum + at(k), a[k]);
         }
+        factor();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!ok(k)) continue;
