@@ -334,7 +334,7 @@ def test_streams_and_workspaces():
         assert all(torch.equal(p, q) for p, q in zip(g, jobs[k % 2][5]))
 
 
-@pytest.mark.parametrize('m,n', [(5, 136), (3000, 700), (64, 5003)])
+@pytest.mark.parametrize('m,n', [(5, 136), (3000, 700), (64, 5003), (1100, 8200)])
 def test_captured_and_replayed(m, n):
     from ultra_amd.ranking_model import layer_norm, layer_norm_backward, layer_norm_workspace
     x, dy = rows(m, n, torch.float32, 1)[0], rows(m, n, torch.float32, 2)[0]
@@ -360,6 +360,34 @@ def test_captured_and_replayed(m, n):
         step()
         assert all(torch.equal(p, q) for p, q in zip(got, (y, stats, dx, dg, db)))
         torch.cuda.synchronize()
+
+
+def test_what_the_c_call_leaves_out():
+    """No statistics, no weights, one row whose stride is nonsense, no workspace where none is needed."""
+    from ultra_amd import _lib
+    lib, st = _lib.lib(), _lib.current_stream()
+    x, _ = rows(1, 700, torch.float16, 1)
+    gamma, _ = weights(700, torch.float16, 2)
+    y = torch.empty_like(x)
+    for ld in (0, -5, 3, 1 << 39):
+        y.fill_(0)
+        assert lib.ultr_layer_norm_forward(x.data_ptr(), ld, gamma.data_ptr(), None, 1, 700, EPS, _lib.DTYPE_F16, _lib.DTYPE_F16,
+                                           y.data_ptr(), ld, None, st) == 0
+        ry, rs, ty, _ = ref_forward(x, gamma, None)
+        within(y, ry, ty, 'y')
+    stats = rs.float()
+    dx, db = torch.empty_like(x), torch.empty(700, dtype=torch.float16, device='cuda')
+    assert lib.ultr_layer_norm_workspace_bytes(1, 700) == 0
+    assert lib.ultr_layer_norm_backward(y.data_ptr(), 0, x.data_ptr(), -1, stats.data_ptr(), None, 1, 700, _lib.DTYPE_F16, _lib.DTYPE_F16,
+                                        dx.data_ptr(), 0, None, db.data_ptr(), None, st) == 0
+    rx, _, rb, tx, _, tb = ref_backward(y, x, stats, None)
+    within(dx, rx, tx, 'dx')
+    within(db, rb, tb + half_step(torch.float16, rb), 'd_beta')
+    # no rows: weight gradients are zero, nothing else is touched
+    db.fill_(3)
+    assert lib.ultr_layer_norm_backward(None, 0, None, 0, None, None, 0, 700, _lib.DTYPE_F16, _lib.DTYPE_F16, None, 0, None, db.data_ptr(),
+                                        None, st) == 0
+    assert not db.any()
 
 
 def test_python_refusals():

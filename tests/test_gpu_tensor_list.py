@@ -256,6 +256,38 @@ def test_a_graph_outlives_the_list_it_was_captured_with():
     del waste
 
 
+def test_what_the_c_calls_leave_out():
+    """No norm wanted, none formed, an empty list, scalars, a plan laid out by the C call itself."""
+    import ctypes
+    from ultra_amd import _lib
+    from ultra_amd.learning_algorithm import GradientTensors
+    lib, st = _lib.lib(), _lib.current_stream()
+    grads, params = tensors([4099, 3], (F16, F32), 1), tensors([4099, 3], (F32,), 2)
+    out = [torch.empty_like(g) for g in grads]
+    rec = (_lib.UltrTensor * 2)(*[_lib.UltrTensor(g.data_ptr(), o.data_ptr(), p.data_ptr(), None, None, g.numel(), _lib.DTYPE_F16 if g.dtype == F16 else _lib.DTYPE_F32, 0)
+                                  for g, o, p in zip(grads, out, params)])
+    nbytes = lib.ultr_tensors_table_bytes(rec, 2)
+    table = torch.full((nbytes,), 255, dtype=torch.uint8, device='cuda')
+    plan = _lib.UltrTensorPlan()
+    assert lib.ultr_tensors_plan(rec, 2, table.data_ptr(), nbytes, ctypes.byref(plan), st) == 0
+    assert plan.has == 3 and plan.n_tensors == 2 and plan.n_chunks == 3
+    ctypes.memset(rec, 255, ctypes.sizeof(rec))  # the list may be dropped at once
+    want = ref_norm(grads)
+    assert lib.ultr_clip_by_global_norm(ctypes.byref(plan), None, 1.0, want / 4, None, st) == 0
+    for o, g in zip(out, grads):
+        within(o, g.double() / 4, 4 * U * g.double().abs() + half_step(g.dtype, g.double() / 4), 'out')
+    before = [p.double() for p in params]
+    assert lib.ultr_clip_adagrad_tensors(ctypes.byref(plan), None, 1.0, 0.0, 0.0, 0.5, _lib.OPT_SGD, None, st) == 0  # one launch
+    for p, b, g in zip(params, before, grads):
+        within(p, b - 0.5 * g.double(), 4 * U * (b.abs() + g.double().abs()), 'param')
+    assert lib.ultr_clip_adagrad_tensors(ctypes.byref(plan), None, 1.0, 0.0, 1.0, 0.5, _lib.OPT_ADAGRAD, None, st) == -1
+    empty = GradientTensors([], out=[], params=[], accums=[])
+    assert float(empty.global_norm()) == 0 and empty.clip(1.0)[0] == [] and float(empty.clip_adagrad(1.0, 0.1)) == 0
+    scalar, vector = torch.tensor(3.0, device='cuda'), torch.tensor([4.0], device='cuda')
+    got, norm = GradientTensors([scalar, vector]).clip(1.0)
+    assert float(norm) == 5.0 and got[0].shape == () and abs(float(got[0]) - 0.6) <= 1e-7 and abs(float(got[1]) - 0.8) <= 1e-7
+
+
 def test_two_lists_in_flight():
     from ultra_amd.learning_algorithm import GradientTensors
     lists = []

@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(32 * K) layer_norm_dw_sum_kernel(const float* 
   const int col = blockIdx.x * 32 + c;
   float s = 0.f;
   if (col < 2 * N) {
-#pragma unroll 4
+#pragma unroll 8
     for (int p = k; p < P; p += K) s += ws[(long long)p * 2 * N + col];
   }
   part[k][c] = s;
