@@ -36,8 +36,10 @@ static void forward_shape(int N, F&& fn) {
                 Shape<1024, 8, 8>{});
   }
 }
-// Backward: 16 elements a thread, up to the 512 threads of a workgroup; rows that are only held for a moment (FEW) take more.
+// Backward: 16 elements a thread, up to the 512 threads of a workgroup; 16-bit rows then 32 (4096 rows of 16384 bf16: 87 us,
+// 129 in column tiles; 1500 rows: 44 and 54; fp32 spills), and rows that are only held for a moment (FEW) what fits.
 constexpr int kGradWidth = 16 * kGradThreads;
+constexpr int kHeldWidth16 = 2 * kGradWidth;
 constexpr int kFewWidth32 = 32768;  // 16-bit types: every width
 template <typename T, bool FEW, typename F>
 static void grad_shape(int N, F&& fn) {
@@ -50,7 +52,8 @@ static void grad_shape(int N, F&& fn) {
   } else {
     if (N < 8) return fn(Shape<8, 1, 1>{});
     if constexpr (FEW)
-      if (N > kGradWidth) return first_shape(N, fn, Shape<512, 4, 8>{}, Shape<1024, 4, 8>{}, Shape<1024, 8, 8>{});
+      if (N > kHeldWidth16) return first_shape(N, fn, Shape<1024, 4, 8>{}, Shape<1024, 8, 8>{});
+    if (N > kGradWidth) return fn(Shape<512, 4, 8>{});
     first_shape(N, fn, Shape<4, 1, 8>{}, Shape<4, 2, 8>{}, Shape<8, 2, 8>{}, Shape<16, 2, 8>{}, Shape<32, 2, 8>{}, Shape<64, 2, 8>{},
                 Shape<128, 2, 8>{}, Shape<256, 2, 8>{}, Shape<512, 2, 8>{});
   }
@@ -60,7 +63,8 @@ static void grad_shape(int N, F&& fn) {
 enum GradPass { kFew, kHeld, kWide };
 static GradPass grad_pass(long long M, int N, int x_dtype) {
   if (N <= kGradWidth) return M <= 512 ? kFew : kHeld;
-  return M <= 1024 && (x_dtype != ULTR_DTYPE_F32 || N <= kFewWidth32) ? kFew : kWide;
+  if (M <= 1024 && (x_dtype != ULTR_DTYPE_F32 || N <= kFewWidth32)) return kFew;
+  return x_dtype != ULTR_DTYPE_F32 && N <= kHeldWidth16 ? kHeld : kWide;
 }
 // Row groups' workgroups of the held pass = its partial rows.  One per CU; half of them while each would get fewer than 3
 // turns (the partial rows cost more than the idle CUs: 1000 rows of 4096 bf16 14.3 us with 128, 15.4 with 256; 3000 rows

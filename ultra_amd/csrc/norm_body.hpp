@@ -137,9 +137,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 // Backward, rows that a workgroup holds.  HBM-bound: two reads and one write of the matrix.  A workgroup walks over the rows,
 // kGradThreads / TPR at a time, with the next ones on their way while these are worked on; a thread keeps its columns' share
 // of d_gamma and d_beta in registers over the whole walk.  What the row groups of a workgroup hold meets in LDS at the end
-// and leaves as one partial row.  16 elements a thread and 512 threads:
-// 16384 rows of 4096 bf16 77 us = 5.2 TB/s; with 1024 threads the registers spill (102 us), without the prefetch 8192 rows
-// of 8192 take 100 us against 81.  Nothing needs x and dy after this, so they do not stay in the caches (40960 rows of 512
+// and leaves as one partial row.  16 elements a thread and 512 threads: 16384 rows of 4096 bf16 74 us = 5.4 TB/s; with 1024
+// threads the registers spill (102 us), without the prefetch 8192 rows of 8192 take 100 us against 81.  Nothing needs x and dy after this, so they do not stay in the caches (40960 rows of 512
 // fp32: 45 us, 50 with plain loads) -- but for odd widths, whose pieces share cache lines with their neighbours.
 template <typename T, typename W, int TPR, int C, int V, bool TAIL>
 __global__ void __launch_bounds__(kGradThreads)
@@ -247,7 +246,8 @@ __global__ void __launch_bounds__(kGradThreads)
 // Backward of few rows, in one launch and without a workspace: d_gamma and d_beta need the statistics, not dx, so the last
 // workgroups of the grid form dx, whole rows in registers, while the first ones sum columns.  Everything is read twice,
 // mostly out of a cache the second time; the pass above writes and re-reads partial rows instead, and takes a second launch.
-// 100 rows of 4096 bf16: 5.5 us, 9.0 the other way; 512 rows: 9.7 and 11.8; 1000 rows: 13 and 14.6, and beyond it loses.
+// 100 rows of 4096 bf16: 5.5 us, 9.0 the other way; 512 rows: 9.7 and 11.8; beyond, narrow rows lose by it (1000 rows of 136
+// fp32: 12.4 and 6.5) and rows of more than 8192 gain up to about 1024 (777 rows of 12345 bf16: 22 us, 29 in column tiles).
 //
 // Columns: the threads of a workgroup as `rt` row threads times NT / rt threads of V columns each (8 at least: 128 bytes).
 template <typename T, typename W, int V, bool TAIL, int NT>
@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR)
 // Backward, rows wider than that: the two sums of every row first, then a pass in which a workgroup owns a column tile and
 // a slice of the rows.  Reads the matrices twice; nothing but the two sums crosses threads.  The slice is the fastest index
 // of that pass's grid and a multiple of 8, so that (workgroups go to the 8 XCDs in turn) an XCD meets the rows whose sums
-// it formed, the last ones first: its L2 may still hold them (4096 rows of 16384 bf16: 124 us, other orders 130).
+// it formed, the last ones first: its L2 may still hold them (512 rows of 65536 bf16 in
+// this pass: 77 us, other orders 81).
 template <typename T, typename W, int V, bool TAIL, int NT>
 __global__ void __launch_bounds__(NT)
     layer_norm_row_sums_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,
