@@ -86,7 +86,8 @@ def within(got, want, tol, what):
 
 SIZES = [(1, 1), (3, 1), (1, 2), (2, 3), (2, 7), (5, 8), (9, 15), (7, 33), (64, 63), (4, 64), (33, 65), (10, 136), (17, 255), (6, 256),
          (9, 700), (3, 1023), (2, 1024), (5, 1025), (3, 2047), (3, 2048), (3, 2049), (2, 4096), (2, 4099), (2, 5003), (2, 8192),
-         (1, 8193), (2, 12345), (2, 16384), (2, 16385), (1, 32768), (1, 32769), (2, 65535), (1, 65536)]
+         (1, 8193), (2, 12345), (2, 16384), (2, 16385), (1, 32768), (1, 32769), (2, 65535), (1, 65536),
+         (5, 40), (5, 57), (5, 100), (5, 200), (5, 400), (3, 900), (3, 1592), (3, 3300), (3, 3585)]
 
 
 @pytest.mark.parametrize('m,n', SIZES)

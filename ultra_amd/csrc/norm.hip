@@ -20,8 +20,10 @@ template <typename... S, typename F>
 static void first_shape(int N, F&& fn, S... shapes) {
   (void)((N <= S::TPR * S::C * S::V ? (fn(shapes), true) : false) || ...);
 }
-// Forward: 8 elements a thread until a workgroup is full (two 16-byte pieces of fp32, one of 16-bit types; with 4 or 16 the
-// same widths lose 2 to 10 %), then more.  Rows shorter than one piece: element by element.
+// Forward: two 16-byte pieces a thread until a workgroup is full, then more (fp32: one or four lose 2 to 10 %).  16-bit rows
+// that fill twice the threads with one piece each take those (16384 rows of 4096 bf16, fp32 weights: 50 us, 52 with two
+// pieces); where many threads would be idle they do not (16969 rows of 1052 fp16: 21 us, 17 with two pieces; 1592 of 2048
+// threads' worth: 14.9 and 13.2).  Rows shorter than one piece: element by element.
 template <typename T, typename F>
 static void forward_shape(int N, F&& fn) {
   if constexpr (sizeof(T) == 4) {
@@ -31,9 +33,15 @@ static void forward_shape(int N, F&& fn) {
                 Shape<1024, 16, 4>{});
   } else {
     if (N < 8) return fn(Shape<8, 1, 1>{});
-    first_shape(N, fn, Shape<4, 1, 8>{}, Shape<8, 1, 8>{}, Shape<16, 1, 8>{}, Shape<32, 1, 8>{}, Shape<64, 1, 8>{}, Shape<128, 1, 8>{},
-                Shape<256, 1, 8>{}, Shape<512, 1, 8>{}, Shape<512, 2, 8>{}, Shape<1024, 2, 8>{}, Shape<1024, 4, 8>{},
-                Shape<1024, 8, 8>{});
+    int held = 32;  // entries that a power of two of threads holds with one piece each
+    while (held < N) held *= 2;
+    if (held <= 4096 && 8 * N >= 7 * held)
+      first_shape(N, fn, Shape<4, 1, 8>{}, Shape<8, 1, 8>{}, Shape<16, 1, 8>{}, Shape<32, 1, 8>{}, Shape<64, 1, 8>{}, Shape<128, 1, 8>{},
+                  Shape<256, 1, 8>{}, Shape<512, 1, 8>{});
+    else
+      first_shape(N, fn, Shape<4, 1, 8>{}, Shape<4, 2, 8>{}, Shape<8, 2, 8>{}, Shape<16, 2, 8>{}, Shape<32, 2, 8>{}, Shape<64, 2, 8>{},
+                  Shape<128, 2, 8>{}, Shape<256, 2, 8>{}, Shape<512, 2, 8>{}, Shape<1024, 2, 8>{}, Shape<1024, 4, 8>{},
+                  Shape<1024, 8, 8>{});
   }
 }
 // Backward: 16 elements a thread, up to the 512 threads of a workgroup; 16-bit rows then 32 (4096 rows of 16384 bf16: 87 us,

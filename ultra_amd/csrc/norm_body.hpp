@@ -138,8 +138,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
 // kGradThreads / TPR at a time, with the next ones on their way while these are worked on; a thread keeps its columns' share
 // of d_gamma and d_beta in registers over the whole walk.  What the row groups of a workgroup hold meets in LDS at the end
 // and leaves as one partial row.  16 elements a thread and 512 threads: 16384 rows of 4096 bf16 74 us = 5.4 TB/s; with 1024
-// threads the registers spill (102 us), without the prefetch 8192 rows of 8192 take 100 us against 81.  Nothing needs x and dy after this, so they do not stay in the caches (40960 rows of 512
-// fp32: 45 us, 50 with plain loads) -- but for odd widths, whose pieces share cache lines with their neighbours.
+// threads the registers spill (102 us), without the prefetch 8192 rows of 8192 take 100 us against 81.  Nothing needs x and
+// dy after this, so they do not stay in the caches (40960 rows of 512 fp32: 45 us, 50 with plain loads) -- but for odd
+// widths, whose pieces share cache lines with their neighbours.
 template <typename T, typename W, int TPR, int C, int V, bool TAIL>
 __global__ void __launch_bounds__(kGradThreads)
     layer_norm_grad_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,
@@ -368,8 +369,7 @@ __global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR)
 // Backward, rows wider than that: the two sums of every row first, then a pass in which a workgroup owns a column tile and
 // a slice of the rows.  Reads the matrices twice; nothing but the two sums crosses threads.  The slice is the fastest index
 // of that pass's grid and a multiple of 8, so that (workgroups go to the 8 XCDs in turn) an XCD meets the rows whose sums
-// it formed, the last ones first: its L2 may still hold them (512 rows of 65536 bf16 in
-// this pass: 77 us, other orders 81).
+// it formed, the last ones first: its L2 may still hold them (512 rows of 65536 bf16 in this pass: 77 us, other orders 81).
 template <typename T, typename W, int V, bool TAIL, int NT>
 __global__ void __launch_bounds__(NT)
     layer_norm_row_sums_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,

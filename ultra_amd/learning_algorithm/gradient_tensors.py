@@ -11,6 +11,7 @@ import torch
 
 from .. import _lib
 
+_current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)  # without the lazy-init check
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _REC = np.dtype([('grad', 'u8'), ('out', 'u8'), ('param', 'u8'), ('accum', 'u8'), ('copy', 'u8'), ('n', 'i8'),
                  ('grad_dtype', 'i4'), ('copy_dtype', 'i4')])  # _lib.UltrTensor, filled a column at a time
@@ -92,7 +93,7 @@ class GradientTensors(object):
         self._plan = ctypes.pointer(plan)
 
     def _stream(self):
-        if torch.cuda.current_device() != self._index:
+        if _current_device() != self._index:
             raise ValueError('these tensors live on %s, the current device is cuda:%d' % (self.device, torch.cuda.current_device()))
         return _lib.stream_of(self._index)
 

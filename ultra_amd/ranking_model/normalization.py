@@ -15,6 +15,7 @@ from .. import _lib
 from .DNN import LN_EPS
 
 _F32 = torch.float32
+_current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)  # without the lazy-init check
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
 
@@ -49,7 +50,7 @@ def _input(x):
     code = _DTYPE.get(dtype)
     if code is None:
         raise ValueError('layer norm takes float32, bfloat16 or float16, got %s' % dtype)
-    if device < 0 or device != torch.cuda.current_device():
+    if device < 0 or device != _current_device():
         raise ValueError('layer norm runs on the current device, got a tensor on %s' % x.device)
     return dtype, code, device, x.shape
 
