@@ -557,8 +557,8 @@ int ultr_clip_adagrad3(float* theta, float* acc, const float* grads, long long n
                        float* out_norm_s, const float* sumsq, int n_sumsq, long long n_covered,
                        const float* publish_src, float* publish_dst, int publish_n, void* stream);
 
-/* ---- global norm, clipping and the update over MANY tensors (tf.clip_by_global_norm + apply_gradients over the
- * variable list, dla.py:237-255; ipw_rank.py:155-165) -----------------------------------------------------------------
+/* ---- global norm, clipping and the update over MANY tensors (the clip by the global norm and the optimiser step over
+ * the variable list, dla.py:237-255; ipw_rank.py:155-165) -----------------------------------------------------------------
  * The calls above work on one flat fp32 buffer.  These take a list of separate tensors of any size and alignment:
  * gradients in fp32, bf16 or fp16 and, for the update, fp32 parameters and accumulators, with an optional bf16 / fp16
  * copy of each updated parameter.  The list is laid out once, by ultr_tensors_plan, into a device table that the
@@ -598,7 +598,7 @@ int ultr_global_norm(const UltrTensorPlan* plan_h, const float* denom, float sca
 
 /* out = f * scale * grad for every tensor, f = clip_norm / max(norm, clip_norm) with the norm above (also written to
  * out_norm if that is not NULL).  clip_norm <= 0: f = 1; NaN is refused.  A norm that is not finite makes f NaN, and so every output
- * NaN (tf.clip_by_global_norm).  Needs `out` in every tensor. */
+ * NaN (as the reference's clip does).  Needs `out` in every tensor. */
 int ultr_clip_by_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float clip_norm,
                              float* out_norm, void* stream);
 

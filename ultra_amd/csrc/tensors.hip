@@ -1,5 +1,5 @@
 // Global norm, clipping and the optimiser update over a list of separate tensors.
-// Reference: tf.clip_by_global_norm + apply_gradients over the variable list, dla.py:237-255, ipw_rank.py:155-165.
+// Reference: the clip by the global norm and the optimiser step over the variable list, dla.py:237-255, ipw_rank.py:155-165.
 //   e = scale * g (+ l2 * theta) ; norm = sqrt(sum e^2) ; f = clip / max(norm, clip) ; out = f e, or
 //   acc += (f e)^2, theta -= lr f e / sqrt(acc).
 // The norm is needed before the first output: two passes over the gradients, one launch each.

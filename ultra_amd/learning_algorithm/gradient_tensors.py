@@ -1,6 +1,6 @@
 """Global gradient norm, clipping and the Adagrad / SGD update over many separate tensors.
 
-Reference: tf.clip_by_global_norm + optimizer.apply_gradients over the list of trainable variables (dla.py:237-255,
+Reference: the clip by the global norm and the optimiser step over the list of trainable variables (dla.py:237-255,
 ipw_rank.py:155-165).  The learning algorithms of this package keep their variables in one flat float32 buffer
 (``ultr_clip_adagrad``); a model whose parameters are tensors of their own lists them here, once.
 """
@@ -112,7 +112,7 @@ class GradientTensors(object):
         return self.norm
 
     def clip(self, clip_norm, denom=None, scale=1.0):
-        """-> (out, norm), as tf.clip_by_global_norm: out = scale / denom * g * clip_norm / max(norm, clip_norm).  A norm that
+        """-> (out, norm): out = scale / denom * g * clip_norm / max(norm, clip_norm).  A norm that
         is not finite makes every output NaN; clip_norm <= 0 does not clip."""
         if self.out is None:
             if torch.cuda.is_current_stream_capturing():
