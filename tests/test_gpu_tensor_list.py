@@ -288,6 +288,31 @@ def test_what_the_c_calls_leave_out():
     assert float(norm) == 5.0 and got[0].shape == () and abs(float(got[0]) - 0.6) <= 1e-7 and abs(float(got[1]) - 0.8) <= 1e-7
 
 
+def test_a_scorers_own_parameters_in_a_list():
+    """The fused step streams copies of the weights that its own update keeps current: an update through a list must not leave
+    them stale.  The second model takes the same values through a copy that torch knows of."""
+    from tests.test_gpu_step import PBM, make, settings
+    from tests.util import SyntheticData
+    from ultra_amd.learning_algorithm import GradientTensors
+    data = SyntheticData(300, 10, 24, seed=11)
+    exp = settings('DLA', '', 'hidden_layer_sizes=[64, 32]', Lmax=10, cutoff=10, feed_hparams='click_model_json=%s' % PBM)
+    m1, feed = make('DLA', data, exp, 64)
+    m2, _ = make('DLA', data, exp, 64)
+    assert m1.model.fused_supported(64, 10)
+    batch, _ = feed.get_batch(data, check_validation=True)
+    for m in (m1, m2):
+        m.step(None, batch, False)
+    p = m1.model.params
+    half = p.numel() // 2
+    plan = GradientTensors([torch.randn(half, device='cuda'), torch.randn(p.numel() - half, device='cuda')], params=[p[:half], p[half:]])
+    for _ in range(2):
+        plan.clip_adagrad(0.0, 0.5, grad_strategy='sgd')
+        m2.model.params.copy_(p)
+        for m in (m1, m2):
+            m.step(None, batch, False)
+        assert torch.equal(m1.model.params, m2.model.params)
+
+
 def test_two_lists_in_flight():
     from ultra_amd.learning_algorithm import GradientTensors
     lists = []

@@ -30,7 +30,8 @@ class GradientTensors(object):
     The constructor lays the list out on the device and waits for that; it cannot be captured into a graph.  The tensors
     are held and their CURRENT values are read by every call.  The calls enqueue on torch's current stream, allocate
     nothing once ``out`` is there, never synchronise, and may be captured.  Calls on one object (and replays of graphs that
-    captured them) must be ordered one after the other: they share its partial sums."""
+    captured them) must be ordered one after the other: they share its partial sums.  A replayed graph that updates a DNN
+    scorer's own parameters is not noticed by its fused step: make one eager call after the replays."""
 
     def __init__(self, grads, out=None, params=None, accums=None, copies=None):
         if not torch.cuda.is_available():
@@ -133,6 +134,7 @@ class GradientTensors(object):
         strategy = _STRATEGY.get(grad_strategy)
         if strategy is None:
             raise ValueError("grad_strategy '%s' unknown (ada, sgd)" % grad_strategy)
+        _lib.param_epoch += 1  # a scorer's fused step notices that its parameters may have been among them
         rc = _lib._lib.ultr_clip_adagrad_tensors(self._plan, self._denom(denom), scale, l2, clip_norm, learning_rate, strategy,
                                                  self._norm_ptr, self._stream())
         if rc:

@@ -235,7 +235,7 @@ class DNN(BaseRankingModel):
         ws = self._fused_workspace(B, L)
         # the workspace's transposed weight copies are current iff the last writer of the parameters was the update
         # call that refreshed them (torch bumps the version counter on every in-place write of its own)
-        fresh = self._wt_state == (ws.data_ptr(), self.params._version)
+        fresh = self._wt_state == (ws.data_ptr(), self.params._version, _lib.param_epoch)
         _lib.check(_lib.lib().ultr_dnn_train_fused(
             self.desc, _lib.ptr(self.params), _lib.ptr(table), _lib.ptr(table_stats), int(n_rows), int(table.stride(0)),
             _lib.ptr(docids_lb), int(B), int(L), _lib.ptr(ws), 1 if fresh else 0, _lib.ptr(scores), _lib.ptr(grads),
@@ -248,7 +248,7 @@ class DNN(BaseRankingModel):
         return self._last_fused
 
     def mark_wt_fresh(self, ws):
-        self._wt_state = (ws.data_ptr(), self.params._version)
+        self._wt_state = (ws.data_ptr(), self.params._version, _lib.param_epoch)
 
     def sumsq_count(self):
         return int(_lib.lib().ultr_dnn_sumsq_count(self.desc))
