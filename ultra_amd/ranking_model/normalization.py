@@ -20,9 +20,9 @@ _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.
 
 
 # A call on a few rows costs what its checks cost (a launch is 2.5 us of host time): each reads a tensor's attributes once.
-def _rows(t, name):
-    """(rows, row stride in elements) of a tensor whose last axis is contiguous."""
-    shape, strides = t.shape, t.stride()
+def _rows(t, shape, name):
+    """(rows, row stride in elements) of a tensor of this shape whose last axis is contiguous."""
+    strides = t.stride()
     if len(strides) == 2 and strides[1] == 1 and shape[1]:
         return shape[0], strides[0]
     if not strides or shape[-1] == 0:
@@ -57,15 +57,15 @@ def _input(x):
 
 def _like(t, name, device, dtype, shape):
     """Row stride of a matrix that must be like x."""
-    if t.dtype != dtype or t.shape != shape or t.get_device() != device:
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
         raise ValueError('%s: %s %s on cuda:%d expected, got %s %s on %s' % (name, dtype, tuple(shape), device, t.dtype, tuple(t.shape), t.device))
-    return _rows(t, name)[1]
+    return _rows(t, shape, name)[1]
 
 
 def _weight(w, name, dtype, n, device, code):
     """dtype code of a weight vector; code: what the others have, None so far."""
     t = w.dtype
-    got = _DTYPE[t] if t == _F32 or t == dtype else None
+    got = _DTYPE[t] if t is _F32 or t is dtype else None
     if got is None or w.shape != (n,) or not w.is_contiguous() or w.get_device() != device:
         raise ValueError('%s: %d contiguous entries of float32 or %s on cuda:%d expected, got %s %s on %s'
                          % (name, n, dtype, device, t, tuple(w.shape), w.device))
@@ -75,7 +75,8 @@ def _weight(w, name, dtype, n, device, code):
 
 
 def _stats(stats, shape, device):
-    if stats.dtype != _F32 or stats.shape != shape[:-1] + (2,) or not stats.is_contiguous() or stats.get_device() != device:
+    want = (shape[0], 2) if len(shape) == 2 else shape[:-1] + (2,)
+    if stats.dtype is not _F32 or stats.shape != want or not stats.is_contiguous() or stats.get_device() != device:
         raise ValueError('stats: contiguous float32 %s on cuda:%d expected, got %s %s on %s'
                          % (tuple(shape[:-1]) + (2,), device, stats.dtype, tuple(stats.shape), stats.device))
 
@@ -84,7 +85,7 @@ def layer_norm(x, gamma=None, beta=None, eps=LN_EPS, out=None, stats=None):
     """-> (out, stats): out = (x - mean) * rstd * gamma + beta over the last axis, stats[..., 0:2] = (mean, rstd) in float32
     (the layout of ``feature_row_stats``).  ``out`` may be x itself; ``out`` / ``stats`` are allocated when not given."""
     dtype, code, device, shape = _input(x)
-    m, ldx = _rows(x, 'x')
+    m, ldx = _rows(x, shape, 'x')
     n = shape[-1]
     w = g = b = None
     if gamma is not None:
@@ -125,7 +126,7 @@ def layer_norm_backward(d_out, x, stats, gamma=None, d_x=None, d_gamma=None, d_b
     ``need``: which of the three are wanted; the others come back as None.  Gradients are written, not added to;
     d_gamma / d_beta have gamma's type (float32 without gamma) unless given.  d_x must not share memory with d_out or x."""
     dtype, code, device, shape = _input(x)
-    m, ldx = _rows(x, 'x')
+    m, ldx = _rows(x, shape, 'x')
     n = shape[-1]
     lddy = _like(d_out, 'd_out', device, dtype, shape)
     _stats(stats, shape, device)
