@@ -593,7 +593,9 @@ int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, void* table, l
 
 /* out_norm[0] = sqrt(sum over all tensors of (scale * g)^2), scale = scale_const / denom[0] (denom NULL: scale_const),
  * as ultr_clip_adagrad scales.  The products are fp32, their squares are summed in 64 bits in an order fixed by the
- * plan, so the norm neither overflows nor vanishes before fp32 itself does; an empty list gives 0. */
+ * plan, so the norm neither overflows nor vanishes before fp32 itself does; an empty list gives 0.
+ * Here and below: denom is read before anything is written, so it may be out_norm itself or lie in a tensor that the call
+ * writes.  out_norm must lie outside the list's tensors and its table. */
 int ultr_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float* out_norm, void* stream);
 
 /* out = f * scale * grad for every tensor, f = clip_norm / max(norm, clip_norm) with the norm above (also written to

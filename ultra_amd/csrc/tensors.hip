@@ -33,13 +33,15 @@ struct ChunkRec {  // what one chunk needs: its tensor's pointers, moved to its 
 };
 static_assert(sizeof(ChunkRec) == 48, "read as 12 words");
 
-// Table: partial sums of the norm | a record per chunk.  One dependent load from a workgroup's number to its data; 48 bytes
-// for the 8 KB or more that a full chunk moves.
+// Table: partial sums of the norm | the scale | a record per chunk.  One dependent load from a workgroup's number to its data;
+// 48 bytes for the 8 KB or more that a full chunk moves.
 constexpr long long kPartialBytes = kTMaxBlocks * sizeof(double);
-static long long table_bytes_of(long long n_chunks) { return kPartialBytes + n_chunks * (long long)sizeof(ChunkRec); }
+constexpr long long kHeadBytes = kPartialBytes + 16;
+static long long table_bytes_of(long long n_chunks) { return kHeadBytes + n_chunks * (long long)sizeof(ChunkRec); }
 
 struct ListView {
   double* partials;
+  float* scale;  // what the first pass made of denom: the second one may be overwriting that memory
   const ChunkRec* chunks;
   long long n_chunks;
 };
@@ -186,6 +188,7 @@ template <bool STREAM>
 __global__ void __launch_bounds__(kTThreads) tensors_sumsq_kernel(ListView l, const float* denom, float scale_const, float l2) {
   __shared__ double red[kTThreads / 64];
   const float sc = scale_of(denom, scale_const);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *l.scale = sc;
   double acc = 0.0;
   // whole turns of the grid, so that a chunk belongs to the same workgroup in both passes
   const long long past = STREAM ? max(l.n_chunks - kKeepChunks, 0ll) / gridDim.x * gridDim.x : 0;
@@ -208,10 +211,10 @@ __global__ void __launch_bounds__(kTThreads) tensors_norm_kernel(const double* p
 }
 
 template <bool STREAM>
-__global__ void __launch_bounds__(kTThreads) tensors_clip_kernel(ListView l, int n_partials, const float* denom,
-                                                                 float scale_const, float clip_norm, float* out_norm) {
+__global__ void __launch_bounds__(kTThreads) tensors_clip_kernel(ListView l, int n_partials, float clip_norm,
+                                                                 float* out_norm) {
   __shared__ double red[kTThreads / 64];
-  const float sc = scale_of(denom, scale_const);
+  const float sc = *l.scale;
   float f = 1.f;
   bool pending = true;
   auto factor = [&] {  // the norm, once, with the first chunk's elements on their way; every thread comes here
@@ -247,11 +250,11 @@ __global__ void __launch_bounds__(kTThreads) tensors_clip_kernel(ListView l, int
 
 // Second pass of the update.  HBM-bound: reads gradient, parameter and accumulator, writes the last two and the copy.
 template <bool STREAM>
-__global__ void __launch_bounds__(kTThreads) tensors_update_kernel(ListView l, int n_partials, const float* denom,
+__global__ void __launch_bounds__(kTThreads) tensors_update_kernel(ListView l, int n_partials, bool scaled,
                                                                    float scale_const, float l2, float clip_norm, float lr,
                                                                    int strategy, float* out_norm) {
   __shared__ double red[kTThreads / 64];
-  const float sc = scale_of(denom, scale_const);
+  const float sc = scaled ? *l.scale : scale_const;
   float f = 1.f;
   bool pending = n_partials > 0;
   auto factor = [&] {  // as above
@@ -372,21 +375,29 @@ static int check_plan(const char* who, const UltrTensorPlan* p, int need, float 
 }
 static ListView view_of(const UltrTensorPlan* p) {
   char* b = static_cast<char*>(p->table);
-  return ListView{reinterpret_cast<double*>(b), reinterpret_cast<const ChunkRec*>(b + kPartialBytes), p->n_chunks};
+  return ListView{reinterpret_cast<double*>(b), reinterpret_cast<float*>(b + kPartialBytes), reinterpret_cast<const ChunkRec*>(b + kHeadBytes), p->n_chunks};
 }
 static bool streams(const ListView& l) { return l.n_chunks > kStreamChunks; }
 static int pass_blocks(long long n_chunks) { return (int)std::min<long long>(n_chunks, kTMaxBlocks); }
 
-// First pass: partial sums into the table.  Returns their number (0 for a list without elements) or an error.
-static int launch_sumsq(const ListView& l, const float* denom, float scale_const, float l2, hipStream_t s) {
-  const int nb = pass_blocks(l.n_chunks);
-  if (nb == 0) return 0;
+static int launch_sumsq_blocks(const ListView& l, int nb, const float* denom, float scale_const, float l2, hipStream_t s) {
   {
     ProfScope prof_("tensors_sumsq_kernel", s);
     hipLaunchKernelGGL(streams(l) ? tensors_sumsq_kernel<true> : tensors_sumsq_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, denom, scale_const, l2);
   }
-  const int rc = check_launch("tensors_sumsq_kernel");
+  return check_launch("tensors_sumsq_kernel");
+}
+// First pass: partial sums and the scale into the table.  Returns their number (0 for a list without elements) or an error.
+static int launch_sumsq(const ListView& l, const float* denom, float scale_const, float l2, hipStream_t s) {
+  const int nb = pass_blocks(l.n_chunks);
+  if (nb == 0) return 0;
+  const int rc = launch_sumsq_blocks(l, nb, denom, scale_const, l2, s);
   return rc ? rc : nb;
+}
+// The scale alone, for an update that forms no norm: the first pass over no chunk at all.
+static int launch_scale(ListView l, const float* denom, float scale_const, hipStream_t s) {
+  l.n_chunks = 0;
+  return launch_sumsq_blocks(l, 1, denom, scale_const, 0.f, s);
 }
 static int launch_norm(const ListView& l, int n_partials, float* out_norm, hipStream_t s) {
   {
@@ -424,7 +435,7 @@ extern "C" int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, voi
   }
   if (rc) return rc;
   int has = 7;
-  ChunkRec* recs = reinterpret_cast<ChunkRec*>(static_cast<char*>(table) + kPartialBytes);
+  ChunkRec* recs = reinterpret_cast<ChunkRec*>(static_cast<char*>(table) + kHeadBytes);
   long long chunk = 0;
   for (int t0 = 0; t0 < n_tensors; t0 += kFillTensors) {
     FillArgs a{};
@@ -472,7 +483,7 @@ extern "C" int ultr_clip_by_global_norm(const UltrTensorPlan* plan_h, const floa
   if (nb == 0) return out_norm ? launch_norm(l, 0, out_norm, s) : ULTR_OK;
   {
     ProfScope prof_("tensors_clip_kernel", s);
-    hipLaunchKernelGGL(streams(l) ? tensors_clip_kernel<true> : tensors_clip_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, nb, denom, scale_const, clip_norm, out_norm);
+    hipLaunchKernelGGL(streams(l) ? tensors_clip_kernel<true> : tensors_clip_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, nb, clip_norm, out_norm);
   }
   return check_launch("tensors_clip_kernel");
 }
@@ -492,9 +503,13 @@ extern "C" int ultr_clip_adagrad_tensors(const UltrTensorPlan* plan_h, const flo
   }
   const int nb = pass_blocks(l.n_chunks);
   if (nb == 0) return out_norm ? launch_norm(l, 0, out_norm, s) : ULTR_OK;
+  if (np == 0 && denom) {
+    rc = launch_scale(l, denom, scale_const, s);
+    if (rc) return rc;
+  }
   {
     ProfScope prof_("tensors_update_kernel", s);
-    hipLaunchKernelGGL(streams(l) ? tensors_update_kernel<true> : tensors_update_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, np, denom, scale_const, l2, clip_norm, lr,
+    hipLaunchKernelGGL(streams(l) ? tensors_update_kernel<true> : tensors_update_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, np, np > 0 || denom, scale_const, l2, clip_norm, lr,
                        strategy, out_norm);
   }
   return check_launch("tensors_update_kernel");
