@@ -607,7 +607,8 @@ int ultr_clip_by_global_norm(const UltrTensorPlan* plan_h, const float* denom, f
 /* The update of ultr_clip_adagrad over the list: e = scale * g + l2 * theta, norm over all e (0 with clip_norm <= 0 and
  * out_norm NULL: not formed), e *= f, Adagrad: acc += e^2, theta -= lr * e / sqrt(acc); SGD: theta -= lr * e; then
  * copy = theta rounded to copy_dtype.  Gradients are left as they are.  Needs `param` in every tensor, and `accum` for
- * Adagrad.  f as above: a norm that is not finite makes every updated value NaN when clip_norm > 0. */
+ * Adagrad.  f as above: a norm that is not finite makes every updated value NaN when clip_norm > 0.  If it writes a
+ * scorer's parameters, the scorer's next ultr_dnn_train_fused call takes wt_fresh = 0. */
 int ultr_clip_adagrad_tensors(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float l2,
                               float clip_norm, float lr, int strategy, float* out_norm, void* stream);
 

@@ -55,3 +55,81 @@ def test_a_denominator_that_the_call_overwrites():
         assert float(one) == 8.0
         for role in got:
             assert all(torch.equal(a, b) for a, b in zip(got[role], want[role])), (where, role)
+
+
+def scorers(count):
+    """Equal small DNN scorers under DLA, one batch, each stepped twice: their fused steps have run and may keep weight copies."""
+    from tests.test_gpu_step import PBM, make, settings
+    from tests.util import SyntheticData
+    data = SyntheticData(300, 10, 24, seed=11)
+    exp = settings('DLA', '', 'hidden_layer_sizes=[64, 32]', Lmax=10, cutoff=10, feed_hparams='click_model_json=%s' % PBM)
+    made = [make('DLA', data, exp, 64) for _ in range(count)]
+    batch, _ = made[0][1].get_batch(data, check_validation=True)
+    models = [m for m, _ in made]
+    for m in models:
+        assert m.model.fused_supported(64, 10)
+        for _ in range(2):
+            m.step(None, batch, False)
+    return models, batch, [f for _, f in made]
+
+
+def list_over(model):
+    from ultra_amd.learning_algorithm import GradientTensors
+    p = model.model.params
+    half = p.numel() // 2
+    gen = torch.Generator(device='cuda').manual_seed(5)
+    grads = [torch.randn(n, generator=gen, device='cuda') for n in (half, p.numel() - half)]
+    return GradientTensors(grads, params=[p[:half], p[half:]])
+
+
+def test_a_replayed_update_of_a_scorers_parameters():
+    """The graph writes the parameters, nothing else tells the scorer.  m2 takes the values through a copy that torch counts."""
+    (m1, m2), batch, _feeds = scorers(2)
+    plan = list_over(m1)
+    plan.clip_adagrad(0.0, 0.5, grad_strategy='sgd')
+    m2.model.params.copy_(m1.model.params)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        plan.clip_adagrad(0.0, 0.5, grad_strategy='sgd')
+    for m in (m1, m2):
+        m.step(None, batch, False)
+    for _ in range(3):
+        graph.replay()
+        m2.model.params.copy_(m1.model.params)
+        for m in (m1, m2):
+            m.step(None, batch, False)
+        assert torch.equal(m1.model.params, m2.model.params)
+
+
+def test_an_update_between_replays_of_a_scorers_step():
+    (m1, m2), batch, _feeds = scorers(2)
+    plan = list_over(m1)
+    for m in (m1, m2):
+        m.enable_graph_replay(True)
+        m.step(None, batch, False)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m1.step(None, batch, False)
+    for _ in range(3):
+        plan.clip_adagrad(0.0, 0.5, grad_strategy='sgd')
+        m2.model.params.copy_(m1.model.params)
+        graph.replay()
+        m2.step(None, batch, False)
+        torch.cuda.synchronize()
+        assert torch.equal(m1.model.params, m2.model.params)
+
+
+def test_a_list_over_the_parameters_of_a_captured_step():
+    (m1, m2), batch, _feeds = scorers(2)
+    m1.enable_graph_replay(True)
+    m1.step(None, batch, False)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        m1.step(None, batch, False)
+    with pytest.raises(RuntimeError, match='before capturing'):
+        list_over(m1)
+    list_over(m2)  # of which no step was captured
+    assert m1.model._wt_kept and not m2.model._wt_kept

@@ -164,10 +164,6 @@ SIGNATURES = {
 
 _lib = None
 
-# Counts the updates of parameter tensors that anything but a learning algorithm made through the library (the C calls leave
-# torch's version counters alone): what was derived from a scorer's parameters is current only if this has not moved.
-param_epoch = 0
-
 
 def lib():
     """Load libultr_hip.so (once).  Fails loudly: the HIP library IS the implementation."""

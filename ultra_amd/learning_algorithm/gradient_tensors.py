@@ -10,6 +10,7 @@ import numpy as np
 import torch
 
 from .. import _lib
+from ..ranking_model.DNN import parameters_written
 
 _current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)  # without the lazy-init check
 _DTYPE = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
@@ -30,8 +31,11 @@ class GradientTensors(object):
     The constructor lays the list out on the device and waits for that; it cannot be captured into a graph.  The tensors
     are held and their CURRENT values are read by every call.  The calls enqueue on torch's current stream, allocate
     nothing once ``out`` is there, never synchronise, and may be captured.  Calls on one object (and replays of graphs that
-    captured them) must be ordered one after the other: they share its partial sums.  A replayed graph that updates a DNN
-    scorer's own parameters is not noticed by its fused step: make one eager call after the replays."""
+    captured them) must be ordered one after the other: they share its partial sums.
+
+    A list may write a DNN scorer's own parameters, eagerly or in replayed graphs: from its construction on the scorer's
+    fused step forms its transposed weight copies anew every time (other scorers keep theirs).  Such a list has to be built
+    before a training step of that scorer is captured; afterwards it is refused with a RuntimeError."""
 
     def __init__(self, grads, out=None, params=None, accums=None, copies=None):
         if not torch.cuda.is_available():
@@ -89,9 +93,21 @@ class GradientTensors(object):
         self._tables.append(table)  # an earlier one stays: a captured graph may read it
         plan = _lib.UltrTensorPlan()
         _lib.check(lib.ultr_tensors_plan(ptr, n, _lib.ptr(table), nbytes, plan, _lib.current_stream()), 'ultr_tensors_plan')
+        self._tell_scorers(rec)
         # whichever stream uses the plan later finds it written
         torch.cuda.current_stream().synchronize()
         self._plan = ctypes.pointer(plan)
+
+    @staticmethod
+    def _tell_scorers(rec):
+        """The scorers learn which memory the calls on this list write."""
+        size = np.array([4, 2, 2], dtype=np.uint64)  # bytes of a DTYPE_*
+        begin, end = [], []
+        for name, each in (('out', size[rec['grad_dtype']]), ('param', 4), ('accum', 4), ('copy', size[rec['copy_dtype']])):
+            there = (rec[name] != 0) & (rec['n'] > 0)
+            begin.append(rec[name][there])
+            end.append((rec[name] + rec['n'].astype(np.uint64) * np.asarray(each, dtype=np.uint64))[there])
+        parameters_written(np.concatenate(begin), np.concatenate(end))
 
     def _stream(self):
         if _current_device() != self._index:
@@ -134,7 +150,6 @@ class GradientTensors(object):
         strategy = _STRATEGY.get(grad_strategy)
         if strategy is None:
             raise ValueError("grad_strategy '%s' unknown (ada, sgd)" % grad_strategy)
-        _lib.param_epoch += 1  # a scorer's fused step notices that its parameters may have been among them
         rc = _lib._lib.ultr_clip_adagrad_tensors(self._plan, self._denom(denom), scale, l2, clip_norm, learning_rate, strategy,
                                                  self._norm_ptr, self._stream())
         if rc:

@@ -10,6 +10,8 @@ multiple of 4 columns) so clip + Adagrad and the data-parallel all-reduce are si
 """
 import ctypes
 import math
+import threading
+import weakref
 
 import numpy as np
 import torch
@@ -19,6 +21,10 @@ from ..utils import hparams as hp
 from .base_ranking_model import BaseRankingModel
 
 LN_EPS = 1e-3  # tf.keras.layers.LayerNormalization default epsilon
+
+
+_scorers = weakref.WeakSet()  # the scorers that have variables
+_scorers_lock = threading.Lock()
 
 
 def _round_up(x, m):
@@ -44,6 +50,8 @@ class DNN(BaseRankingModel):
         self._last = None
         self._last_fused = None
         self._wt_state = None
+        self._wt_kept = True       # what the scorer's own last update left of the fused step's weight copies may be used
+        self._wt_captured = False  # a captured fused step uses it
 
     # ---- variables -------------------------------------------------------------------------
     def layer_shapes(self, feature_size):
@@ -120,6 +128,8 @@ class DNN(BaseRankingModel):
             self._put(host, j, W, b, np.ones(k, np.float32), np.zeros(k, np.float32))
         self.params = torch.from_numpy(host).to(self.device)
         self._name_variables()
+        with _scorers_lock:
+            _scorers.add(self)
         return self.params
 
     def _put(self, host, j, W, b, gamma, beta):
@@ -235,7 +245,9 @@ class DNN(BaseRankingModel):
         ws = self._fused_workspace(B, L)
         # the workspace's transposed weight copies are current iff the last writer of the parameters was the update
         # call that refreshed them (torch bumps the version counter on every in-place write of its own)
-        fresh = self._wt_state == (ws.data_ptr(), self.params._version, _lib.param_epoch)
+        fresh = self._wt_kept and self._wt_state == (ws.data_ptr(), self.params._version)
+        if fresh and not self._wt_captured:
+            self._wt_captured = torch.cuda.is_current_stream_capturing()
         _lib.check(_lib.lib().ultr_dnn_train_fused(
             self.desc, _lib.ptr(self.params), _lib.ptr(table), _lib.ptr(table_stats), int(n_rows), int(table.stride(0)),
             _lib.ptr(docids_lb), int(B), int(L), _lib.ptr(ws), 1 if fresh else 0, _lib.ptr(scores), _lib.ptr(grads),
@@ -248,7 +260,7 @@ class DNN(BaseRankingModel):
         return self._last_fused
 
     def mark_wt_fresh(self, ws):
-        self._wt_state = (ws.data_ptr(), self.params._version, _lib.param_epoch)
+        self._wt_state = (ws.data_ptr(), self.params._version)
 
     def sumsq_count(self):
         return int(_lib.lib().ultr_dnn_sumsq_count(self.desc))
@@ -266,6 +278,22 @@ class DNN(BaseRankingModel):
         docids = torch.arange(L * B, dtype=torch.int32, device=self.device).view(L, B)
         scores = self.forward_lists(table, stats, L * B, docids, is_training=bool(is_training))
         return [scores[l].view(B, 1) for l in range(L)]
+
+
+def parameters_written(begin, end):
+    """Calls that go round a scorer's own update will write the device memory [begin[k], end[k]) (uint64 arrays) whenever they
+    run or a graph replays them, unseen by torch's version counters.  A scorer whose parameters lie in it makes its weight
+    copies anew in every fused step from now on; one of which a graph already holds a step that does not is refused."""
+    with _scorers_lock:
+        scorers = list(_scorers)
+    for s in scorers:
+        lo = s.params.data_ptr()
+        if not ((begin < lo + 4 * s.params.numel()) & (end > lo)).any():
+            continue
+        if s._wt_kept and s._wt_captured:
+            raise RuntimeError("a captured training step of the scorer with these parameters relies on its weight copies: list "
+                               'the tensors before capturing the step')
+        s._wt_kept = False
 
 
 def feature_row_stats(table, feature_size, eps=LN_EPS):
