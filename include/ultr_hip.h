@@ -257,8 +257,10 @@ int ultr_online_sample_click(float tau, const double* rank_uniforms, const int* 
  * x, y: [M][N] of x_dtype (ULTR_DTYPE_F32 / BF16 / F16), rows ldx / ldy ELEMENTS apart (>= N; the entries of a row are
  * contiguous), any alignment of the element type.  gamma, beta: [N] of w_dtype (ULTR_DTYPE_F32 or x_dtype), each may
  * be NULL (1 and 0).  stats: [M][2] fp32, the layout of ultr_ln_row_stats, 8-byte aligned; may be NULL.
- * Everything between load and store is fp32 (entries 1e19 from the mean leave its range when squared); the mean is formed
- * before the variance.  y may be x itself (same pointer
+ * Everything between load and store is fp32 (entries 1e19 from the mean leave its range when squared), but the mean that y and
+ * the variance are formed with is carried in two floats: what it is off by is small against the spread of the row, also
+ * where the row lies far from zero (a constant row gives beta).  stats hold its fp32 rounding, half a step of the MEAN, which is
+ * what the backward pass normalises with.  y may be x itself (same pointer
  * and stride); any other overlap of the two is refused.  M = 0 is a no-op.  A row holding a NaN or an infinity gives
  * NaN in that row only.  1 <= N <= ULTR_MAX_NORM_WIDTH, eps > 0. */
 int ultr_layer_norm_forward(const void* x, long long ldx, const void* gamma, const void* beta, long long M, int N,

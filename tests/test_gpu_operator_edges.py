@@ -4,7 +4,7 @@ implementations these use."""
 import pytest
 import torch
 
-from tests.test_gpu_tensor_list import BF16, F32, U, half_step, ref_norm, tensors, within
+from tests.test_gpu_tensor_list import BF16, F16, F32, U, half_step, ref_norm, tensors, within
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +133,74 @@ def test_a_list_over_the_parameters_of_a_captured_step():
         list_over(m1)
     list_over(m2)  # of which no step was captured
     assert m1.model._wt_kept and not m2.model._wt_kept
+
+
+def ref_norm_rows(x, gamma, beta, eps=1e-3):
+    """y and stats in 64 bits with their tolerances where rows lie far from zero.  D: additions in a row (16 entries a thread, more
+    beyond 8192, then 6 in a wave and 4 between waves).  e_m: what is left of the mean's error.
+    fp32: the first sum is off by delta = (D + 2) u max|x|, the deviations from it sum to its correction, (D + 4) u of their mean
+    size, which is at most s + delta.
+    16 bit: P entries are added in fp32, all of a row up to 2048 (bf16 8192), a wave's share beyond.  If the smallest that is not 0
+    is at least A P / 2^13 (bf16 2^16), A the largest, all of them and their sums are multiples of one step (11 or 8 bits each)
+    below 2^24 steps: exact.  Else two of them are at least A / 2 apart (P <= 4096), the squared deviations of these P are at
+    least A^2 / 8, and their sum is off by at most D u P A; over N / P of them, by Cauchy, that is D u sqrt(8 P) s of the mean.
+    Its quotient leaves as two floats: 4 u^2 of it.
+    The variance: D + 6 roundings of sums of positive terms s^2 + delta^2, and what e_m changes."""
+    xd = x.double()
+    n = x.shape[-1]
+    g = torch.ones(n, dtype=torch.float64, device='cuda') if gamma is None else gamma.double()
+    b = torch.zeros(n, dtype=torch.float64, device='cuda') if beta is None else beta.double()
+    first = xd[:, :1]
+    mean = first + (xd - first).mean(-1, keepdim=True)  # exact for constant rows
+    d = xd - mean
+    var = d.square().mean(-1, keepdim=True)
+    rstd = (var + eps).rsqrt()
+    s, most = var.sqrt(), xd.abs().amax(-1, keepdim=True)
+    dd = max(16, n / 1024) + 10
+    if x.dtype == F32:
+        delta = (dd + 2) * U * most
+        e_m = (dd + 4) * U * (s + delta)
+    else:
+        delta = U * most
+        p = n if n <= (8192 if x.dtype == BF16 else 2048) else 1024 if n <= 8192 else n / 16
+        e_m = dd * U * (8 * p) ** 0.5 * s + 4 * U * U * most
+    e_d = e_m + 2 * U * (d.abs() + delta)
+    rel = ((dd + 6) * U * (var + delta ** 2) + 2 * (s + delta) * e_m + e_m ** 2) / (var + eps)
+    tol_r = rel / 2 + rel ** 2 + 4 * U  # of rstd, relative, while rel < 1
+    y = d * rstd * g + b
+    tol = half_step(x.dtype, y) + g.abs() * rstd * (e_d * (1 + tol_r) + d.abs() * (tol_r + 4 * U)) + U * (y.abs() + (d * rstd * g).abs())
+    return y, torch.cat([mean, rstd], -1), tol, torch.cat([e_m + U * mean.abs(), rstd * tol_r], -1)
+
+
+@pytest.mark.parametrize('m', [9, 2051])  # from 2048 rows on a thread group works on two of them
+@pytest.mark.parametrize('n', [1, 3, 5, 136, 700, 1023, 2048, 5003, 12345, 40001])
+def test_rows_that_hardly_vary_far_from_zero(m, n):
+    """Constant rows, rows of neighbouring values, rows with one entry far out; features before any scaling reach such values."""
+    from ultra_amd.ranking_model import layer_norm
+    from tests.test_gpu_layer_norm import weights
+    if m > 1000 and n > 6000:
+        m = 2049
+    for t, values in ((F32, (123456.7, -1e6, 1e7, 16777217.0, 3e38, 0.1)), (BF16, (1e6, -3e38, 1e-3)), (F16, (65504.0, -777.0))):
+        gen = torch.Generator(device='cuda').manual_seed(n)
+        x = torch.empty((m, n), dtype=t, device='cuda')
+        for k in range(m):
+            if k >= 27:
+                break
+            v = values[k % len(values)]
+            x[k] = v
+            near = (k // len(values)) % 3
+            if near and abs(v) < 1e18 and abs(v) < 65504:
+                step = torch.finfo(t).eps * abs(v)
+                if near == 1:  # up to three steps of the type above it
+                    x[k] += (torch.randint(0, 4, (n,), generator=gen, device='cuda') * step).to(t)
+                else:
+                    x[k] = torch.randn(n, generator=gen, device='cuda').to(t)
+                    x[k, n // 2] = v
+        for k in range(27, m, 27):
+            x[k:k + 27] = x[:min(27, m - k)]
+        gamma, beta = weights(n, F32 if t == F32 else t, 1)
+        y, stats = layer_norm(x, gamma, beta)
+        ry, rs, ty, ts = ref_norm_rows(x, gamma, beta)
+        within(stats, rs, ts, 'stats %s' % t)
+        within(y, ry, ty, 'y %s' % t)
+        assert torch.isfinite(y).all()  # at 3e38 too, where the sum of a row leaves fp32

@@ -169,7 +169,7 @@ extern "C" int ultr_layer_norm_forward(const void* x, long long ldx, const void*
                "%s: y overlaps x without being x", who);
   if (M == 0) return ULTR_OK;
   hipStream_t s = as_stream(stream);
-  const float inv_n = 1.f / (float)N;
+  const double inv_n = 1.0 / N;
   with_types(x_dtype, w_dtype, [&](auto* t, auto* w) {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;

@@ -2,6 +2,8 @@
 #pragma once
 #include "storage.hpp"
 
+#include <type_traits>
+
 namespace ultr {
 
 constexpr int kNThreads = 256;
@@ -30,6 +32,41 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float* red) {
   }
 }
 
+// The same for the forward pass, whose K are many: one lane takes one wave's sum, the lanes of a DPP row (16) add them up, in
+// 32 or 64 bits (A).  A lane that reads every wave's sums by itself holds 16 K of them in registers.
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+  return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xF, 0xF, true),
+                          __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xF, 0xF, true));
+}
+template <int WIDTH>
+__device__ __forceinline__ double group_sum(double v) {
+  static_assert(WIDTH <= 16, "one DPP row");
+  if (WIDTH > 1) v += dpp_f64<0xB1>(v);   // quad_perm [1,0,3,2]
+  if (WIDTH > 2) v += dpp_f64<0x4E>(v);   // quad_perm [2,3,0,1]
+  if (WIDTH > 4) v += dpp_f64<0x141>(v);  // row_half_mirror (quads already uniform)
+  if (WIDTH > 8) v += dpp_f64<0x140>(v);  // row_mirror
+  return v;
+}
+template <int TPR, typename A, int K>
+__device__ __forceinline__ void row_totals(float (&v)[K], A (&total)[K], float* red) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = group_sum<(TPR < 64 ? TPR : 64)>(v[k]);
+  constexpr int W = TPR > 64 ? TPR / 64 : 1;
+  if (W > 1) {
+    const int wave = threadIdx.x >> 6, mine = (wave & ~(W - 1)) + (threadIdx.x & (W - 1));
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[wave * K + k] = v[k];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int k = 0; k < K; ++k) v[k] = red[mine * K + k];
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) total[k] = group_sum<W>((A)v[k]);
+}
+
 // Where a thread's C pieces of V elements lie in a row of N.  With TAIL (N no multiple of V, N >= V) the last piece is moved
 // back to end with the row; its first skip[] elements belong to the piece before it as well: they are left out of sums, and
 // both pieces store the same values for them.  skip >= V: no piece.
@@ -53,15 +90,33 @@ struct Pieces {
 // row otherwise, serve two rows (fp16 rows of 5003 with fp32 weights, 30010 of them: 117 us against 158).  Narrow rows
 // ask for their weights along with the row (136 fp32: 5.0 TB/s against 4.3); in a workgroup of several waves the other
 // workgroups cover that latency and the registers are worth more (8192 fp32, R = 2: 5.6 TB/s against 4.7).
+//
+// The mean is mean[r] + low[r]: an error of a fraction of the row's OFFSET would be the whole variance of a row that hardly
+// varies (a constant row of 1e6, 5003 entries, came out as 0.9).  That costs 0 to 2 % over one fp32 sum, up to 5 % in
+// one-wave rows that the caches hold (40960 x 136 fp32 9.8 us against 9.3, 16969 x 1052 fp16 19.6 against 18.8).
+//   fp32    mean is the fp32 sum's; the second sums give low = sum(x - mean) / N and the variance sum((x - mean)^2) / N - low^2.
+//   16 bit  an fp32 sum is exact for entries of similar size (up to a factor of 4 for 2048 of them with 11 bits or 8192 with 8),
+//           and where they are not their spread is large against its roundings; longer rows meet in 64 bits from wave to wave.  So
+//           low is what the sum's quotient has beyond fp32 and needs no second sum.
+// Sums run in units of 2^kSumShift, so that no row of finite entries overflows.
+//
+// x - mean must mean the same everywhere: the product that makes the mean is not to be fused into it.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+template <typename T>
+constexpr int kSumShift = sizeof(T) == 4 ? 17 : 13;
 template <typename T, typename W, int TPR, int C, int V, bool TAIL, int R>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
-    layer_norm_kernel(const T* x, long long ldx, const W* gamma, const W* beta, long long M, int N, float inv_n, float eps,
+    layer_norm_kernel(const T* x, long long ldx, const W* gamma, const W* beta, long long M, int N, double inv_n, float eps,
                       T* y, long long ldy, float* stats) {
   constexpr int NT = TPR < 256 ? 256 : TPR;
-  constexpr bool EARLY = TPR <= 128;
+  constexpr bool EARLY = TPR <= 128, WIDE = sizeof(T) == 4;
+  constexpr bool EXACT32 = TPR * C * V <= (std::is_same<T, f16_t>::value ? 2048 : 8192);
   typedef typename Piece<T, V>::type PT;
   typedef typename Piece<W, V>::type PW;
-  __shared__ float red[2][R * NT / 64];
+  __shared__ float red[2][2 * R * NT / 64];
   const int lane = threadIdx.x % TPR;
   const long long row0 = ((long long)blockIdx.x * (NT / TPR) + threadIdx.x / TPR) * R;
   const Pieces<TPR, C, V, TAIL> pc(lane, N);
@@ -83,7 +138,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     for (int c = 0; c < C; ++c)
       if (pc.any(c)) weights(c);
   }
-  float mean[R], rstd[R];
+  constexpr int units = 1 << kSumShift<T>;
+  float mean[R], low[R], rstd[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     mean[r] = 0.f;
@@ -91,27 +147,56 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
     for (int c = 0; c < C; ++c) {
       if (!pc.any(c)) continue;
 #pragma unroll
-      for (int j = 0; j < V; ++j) mean[r] += pc.counted(c, j, to_f32(raw[r][c][j]));
+      for (int j = 0; j < V; ++j) mean[r] = fmaf(1.f / units, pc.counted(c, j, to_f32(raw[r][c][j])), mean[r]);
     }
   }
-  row_sums<TPR>(mean, red[0]);
+  if constexpr (WIDE) {
+    row_totals<TPR>(mean, mean, red[0]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) mean[r] = rounded_product(mean[r], (float)(inv_n * units));
+  } else if constexpr (EXACT32) {
+    const double scale = inv_n * units;
+    const float high = (float)scale, rest = (float)(scale - (double)high);
+    float total[R];
+    row_totals<TPR>(mean, total, red[0]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mean[r] = rounded_product(total[r], high);
+      low[r] = fmaf(total[r], rest, fmaf(total[r], high, -mean[r]));
+    }
+  } else {
+    double total[R];
+    row_totals<TPR>(mean, total, red[0]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      total[r] *= inv_n * units;
+      mean[r] = (float)total[r];
+      low[r] = (float)(total[r] - (double)mean[r]);
+    }
+  }
+  float sums[WIDE ? 2 * R : R];  // of the squares, and of the deviations themselves
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    mean[r] *= inv_n;
-    rstd[r] = 0.f;
+    sums[r] = 0.f;
+    if constexpr (WIDE) sums[R + r] = 0.f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       if (!pc.any(c)) continue;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float d = to_f32(raw[r][c][j]) - mean[r];
-        rstd[r] = fmaf(d, pc.counted(c, j, d), rstd[r]);
+        const float d = to_f32(raw[r][c][j]) - mean[r], dc = pc.counted(c, j, d);
+        sums[r] = fmaf(d, dc, sums[r]);
+        if constexpr (WIDE) sums[R + r] += dc;
       }
     }
   }
-  row_sums<TPR>(rstd, red[1]);
+  row_totals<TPR>(sums, sums, red[1]);
 #pragma unroll
-  for (int r = 0; r < R; ++r) rstd[r] = 1.f / sqrtf(fmaf(rstd[r], inv_n, eps));
+  for (int r = 0; r < R; ++r) {
+    if constexpr (WIDE) low[r] = sums[R + r] * (float)inv_n;
+    const float var = fmaf(-low[r], low[r], sums[r] * (float)inv_n);
+    rstd[r] = 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);  // NaN stays
+  }
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     if (!pc.any(c)) continue;
@@ -122,7 +207,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
       float v[V];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        v[j] = (to_f32(raw[r][c][j]) - mean[r]) * rstd[r];
+        v[j] = fmaf(to_f32(raw[r][c][j]) - mean[r], rstd[r], -low[r] * rstd[r]);
         if (gamma) v[j] *= to_f32(g[c][j]);
         if (beta) v[j] += to_f32(b[c][j]);
       }
@@ -131,7 +216,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR)
   }
 #pragma unroll
   for (int r = 0; r < R; ++r)
-    if (lane == 0 && stats && row0 + r < M) *reinterpret_cast<float2*>(stats + 2 * (row0 + r)) = make_float2(mean[r], rstd[r]);
+    if (lane == 0 && stats && row0 + r < M) *reinterpret_cast<float2*>(stats + 2 * (row0 + r)) = make_float2(mean[r] + low[r], rstd[r]);
 }
 
 // Backward, rows that a workgroup holds.  HBM-bound: two reads and one write of the matrix.  A workgroup walks over the rows,
