@@ -204,3 +204,23 @@ def test_rows_that_hardly_vary_far_from_zero(m, n):
         within(stats, rs, ts, 'stats %s' % t)
         within(y, ry, ty, 'y %s' % t)
         assert torch.isfinite(y).all()  # at 3e38 too, where the sum of a row leaves fp32
+
+
+def test_a_list_dropped_while_another_stream_uses_it():
+    from ultra_amd.learning_algorithm import GradientTensors
+    grads = tensors([4096 * 40 + 3, 5], (F32,), 1)
+    want = ref_norm(grads)
+    plan = GradientTensors(grads)
+    table, nbytes, norm = plan._tables[-1].data_ptr(), plan._tables[-1].numel(), plan.norm
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200 * 1000 * 1000)  # about 0.1 s
+        plan.global_norm()
+    done = side.record_event()
+    del plan
+    others = [torch.full((nbytes,), 255, dtype=torch.uint8, device='cuda') for _ in range(8)]
+    if not done.query():
+        assert all(t.data_ptr() != table for t in others)
+    torch.cuda.synchronize()
+    assert abs(float(norm) - want) <= 4 * U * want

@@ -31,7 +31,8 @@ class GradientTensors(object):
     The constructor lays the list out on the device and waits for that; it cannot be captured into a graph.  The tensors
     are held and their CURRENT values are read by every call.  The calls enqueue on torch's current stream, allocate
     nothing once ``out`` is there, never synchronise, and may be captured.  Calls on one object (and replays of graphs that
-    captured them) must be ordered one after the other: they share its partial sums.
+    captured them) must be ordered one after the other: they share its partial sums.  The object may be dropped while eager
+    calls are in flight, on any stream; it has to outlive the graphs that captured its calls, which read its table.
 
     A list may write a DNN scorer's own parameters, eagerly or in replayed graphs: from its construction on the scorer's
     fused step forms its transposed weight copies anew every time (other scorers keep theirs).  Such a list has to be built
@@ -91,6 +92,7 @@ class GradientTensors(object):
             raise _lib.UltrError(lib.ultr_last_error().decode())
         table = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self._tables.append(table)  # an earlier one stays: a captured graph may read it
+        self._streams = set()  # that have used it
         plan = _lib.UltrTensorPlan()
         _lib.check(lib.ultr_tensors_plan(ptr, n, _lib.ptr(table), nbytes, plan, _lib.current_stream()), 'ultr_tensors_plan')
         self._tell_scorers(rec)
@@ -112,7 +114,14 @@ class GradientTensors(object):
     def _stream(self):
         if _current_device() != self._index:
             raise ValueError('these tensors live on %s, the current device is cuda:%d' % (self.device, torch.cuda.current_device()))
-        return _lib.stream_of(self._index)
+        s = _lib.stream_of(self._index)
+        if s not in self._streams:
+            # dropped with calls in flight on this stream, the list's memory waits for them
+            self._streams.add(s)
+            stream = torch.cuda.current_stream()
+            self._tables[-1].record_stream(stream)
+            self.norm.record_stream(stream)
+        return s
 
     def _denom(self, denom):
         if denom is None:
