@@ -261,7 +261,8 @@ int ultr_online_sample_click(float tau, const double* rank_uniforms, const int* 
  * the variance are formed with is carried in two floats: what it is off by is small against the spread of the row, also
  * where the row lies far from zero (a constant row gives beta).  stats hold its fp32 rounding, half a step of the MEAN, which is
  * what the backward pass normalises with.  y may be x itself (same pointer
- * and stride); any other overlap of the two is refused.  M = 0 is a no-op.  A row holding a NaN or an infinity gives
+ * and stride) or lie between its rows (other columns of one table); any other overlap of y or stats with an argument is
+ * refused.  M = 0 is a no-op.  A row holding a NaN or an infinity gives
  * NaN in that row only.  1 <= N <= ULTR_MAX_NORM_WIDTH, eps > 0. */
 int ultr_layer_norm_forward(const void* x, long long ldx, const void* gamma, const void* beta, long long M, int N,
                             float eps, int x_dtype, int w_dtype, void* y, long long ldy, float* stats, void* stream);
@@ -269,8 +270,8 @@ int ultr_layer_norm_forward(const void* x, long long ldx, const void* gamma, con
 /* Its gradient.  With xh = (x - mean) * rstd from the forward pass's stats and g = dy * gamma:
  *   dx = rstd * (g - mean_N(g) - xh * mean_N(g * xh)) ;  d_gamma = sum_m dy * xh ;  d_beta = sum_m dy
  * dy, dx as x above (lddy, lddx); d_gamma, d_beta: [N] of w_dtype, written, not added to (zeros when M = 0).
- * dx, d_gamma and d_beta may each be NULL (not wanted), not all of them.  No output may overlap an input or another output
- * (checked for dx against x and dy, and among gamma, d_gamma, d_beta).
+ * dx, d_gamma and d_beta may each be NULL (not wanted), not all of them.  No output and no byte of ws that is needed may
+ * overlap an input or another output; rows that lie between each other's, with one stride, do not overlap.
  * The sums over rows are fp32 in an order that depends on (M, N, types) only: equal calls give equal bits.
  * ws: ultr_layer_norm_workspace_bytes(M, N) bytes, 16-byte aligned, contents irrelevant before and after the call; may
  * be NULL when that is 0, or for dx alone at N <= 8192.  Two calls in flight need a workspace each. */

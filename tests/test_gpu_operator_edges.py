@@ -224,3 +224,43 @@ def test_a_list_dropped_while_another_stream_uses_it():
         assert all(t.data_ptr() != table for t in others)
     torch.cuda.synchronize()
     assert abs(float(norm) - want) <= 4 * U * want
+
+
+@pytest.mark.parametrize('t', [F32, BF16])
+@pytest.mark.parametrize('m,n', [(7, 5), (3000, 136), (40, 1030), (1100, 8201)])
+def test_columns_of_one_table(t, m, n):
+    """x, the output and the gradients side by side in one table: no rows overlap."""
+    from tests.test_gpu_layer_norm import ref_backward, ref_forward, weights
+    from ultra_amd.ranking_model import layer_norm, layer_norm_backward
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    table = torch.randn((m, 4 * n + 3), generator=gen, device='cuda').to(t)
+    x, dy, y, dx = (table[:, a:a + n] for a in (1, n + 1, 2 * n + 2, 3 * n + 2))
+    gamma, beta = weights(n, F32, 2)
+    before = table.clone()
+    got, stats = layer_norm(x, gamma, beta, out=y)
+    ry, _, ty, _ = ref_forward(before[:, 1:1 + n], gamma, beta)
+    within(got, ry, ty, 'y')
+    _, dg, db = layer_norm_backward(dy, x, stats, gamma, d_x=dx)
+    rx, rg, rb, tx, tg, tb = ref_backward(before[:, n + 1:2 * n + 1], before[:, 1:1 + n], stats, gamma)
+    within(dx, rx, tx, 'dx')
+    within(dg, rg, tg + half_step(F32, rg), 'd_gamma')
+    within(db, rb, tb + half_step(F32, rb), 'd_beta')
+    for a, b in ((0, 2 * n + 1), (2 * n + 1, 2 * n + 2), (4 * n + 2, 4 * n + 3)):
+        assert torch.equal(table[:, a:b], before[:, a:b])
+    # in the other order, and the workspace behind a matrix that ends before it
+    z = table[:, 0:n]
+    layer_norm(y, out=z)
+    with pytest.raises(Exception, match='overlaps'):
+        layer_norm(x, out=table[:, 2:2 + n])
+
+
+def test_python_calls_that_share_memory():
+    from ultra_amd import _lib
+    from ultra_amd.ranking_model import layer_norm, layer_norm_backward
+    x, dy = torch.randn((6, 8), device='cuda'), torch.randn((6, 8), device='cuda')
+    _, stats = layer_norm(x)
+    for call in (lambda: layer_norm(x, gamma=x[0], out=x), lambda: layer_norm(x, stats=x.view(-1)[:12].view(6, 2)),
+                 lambda: layer_norm_backward(dy, x, stats, d_gamma=dy[1]), lambda: layer_norm_backward(dy, x, stats, gamma=x[2], d_x=x),
+                 lambda: layer_norm_backward(dy, x, stats, d_beta=stats.view(-1)[:8])):
+        with pytest.raises(_lib.UltrError, match='overlaps'):
+            call()

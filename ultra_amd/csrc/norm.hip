@@ -142,12 +142,32 @@ static int check_rows(const char* who, const char* name, const void* p, long lon
   ULTR_REQUIRE(((uintptr_t)p & (dtype_bytes(dtype) - 1)) == 0, ULTR_EINVAL, "%s: %s is not aligned to its element type", who, name);
   return ULTR_OK;
 }
-static bool rows_overlap(const void* a, long long lda, const void* b, long long ldb, long long M, int N, int dtype) {
-  if (M == 0 || !a || !b) return false;
-  const int e = dtype_bytes(dtype);
-  const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
-  const uintptr_t ea = pa + ((uintptr_t)(M - 1) * lda + N) * e, eb = pb + ((uintptr_t)(M - 1) * ldb + N) * e;
-  return pa < eb && pb < ea;
+// Memory of an argument: rows of `width` bytes, `pitch` bytes apart.
+struct Extent {
+  uint64_t at, end, pitch, width;
+  bool one;  // row
+};
+static Extent vector(const void* p, long long bytes) {
+  const uint64_t at = (uint64_t)(uintptr_t)p;
+  return {at, p ? at + bytes : 0, 0, (uint64_t)bytes, true};  // a null pointer: nothing
+}
+static Extent matrix(const void* p, long long ld, long long M, int N, int dtype) {
+  Extent v = vector(p, M == 0 ? 0 : (long long)N * dtype_bytes(dtype));
+  if (!p || M <= 1) return v;
+  v.one = false;
+  v.pitch = (uint64_t)ld * dtype_bytes(dtype);
+  uint64_t more;
+  if (__builtin_mul_overflow((uint64_t)(M - 1), v.pitch, &more) || __builtin_add_overflow(v.end, more, &v.end)) v.end = UINT64_MAX;
+  return v;
+}
+// Whether the two have a byte in common.  Rows that lie between each other's (columns of one table) do not; of matrices with
+// different pitches nothing but their ends is looked at.
+static bool touch(const Extent& a, const Extent& b) {
+  if (b.at >= a.end || a.at >= b.end) return false;
+  const Extent &f = a.at <= b.at ? a : b, &s = a.at <= b.at ? b : a;  // the first and the second to begin
+  if (f.one || (!s.one && f.pitch != s.pitch)) return true;
+  const uint64_t in = (s.at - f.at) % f.pitch;  // the second begins this far behind a row of the first
+  return in < f.width || (s.at - in + f.pitch < f.end && in + s.width > f.pitch);
 }
 
 }  // namespace ultr
@@ -165,8 +185,13 @@ extern "C" int ultr_layer_norm_forward(const void* x, long long ldx, const void*
   ULTR_REQUIRE(eps > 0.f, ULTR_EINVAL, "%s: eps=%g", who, (double)eps);
   ULTR_REQUIRE((((uintptr_t)gamma | (uintptr_t)beta) & (dtype_bytes(w_dtype) - 1)) == 0 && ((uintptr_t)stats & 7) == 0, ULTR_EINVAL,
                "%s: gamma, beta or stats not aligned", who);
-  ULTR_REQUIRE((x == y && (ldx == ldy || M <= 1)) || !rows_overlap(x, ldx, y, ldy, M, N, x_dtype), ULTR_EINVAL,
-               "%s: y overlaps x without being x", who);
+  const Extent mx = matrix(x, ldx, M, N, x_dtype), my = matrix(y, ldy, M, N, x_dtype);
+  ULTR_REQUIRE((x == y && (ldx == ldy || M <= 1)) || !touch(mx, my), ULTR_EINVAL, "%s: y overlaps x without being x", who);
+  const Extent weights[] = {vector(gamma, (long long)N * dtype_bytes(w_dtype)), vector(beta, (long long)N * dtype_bytes(w_dtype))};
+  const Extent ms = vector(stats, M * 8);
+  bool shared = touch(ms, mx) || touch(ms, my);
+  for (const Extent& w : weights) shared = shared || touch(w, my) || touch(w, ms);
+  ULTR_REQUIRE(!shared, ULTR_EINVAL, "%s: y or stats overlaps another argument", who);
   if (M == 0) return ULTR_OK;
   hipStream_t s = as_stream(stream);
   const double inv_n = 1.0 / N;
@@ -233,17 +258,22 @@ extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const vo
   ULTR_REQUIRE((((uintptr_t)gamma | (uintptr_t)d_gamma | (uintptr_t)d_beta) & (dtype_bytes(w_dtype) - 1)) == 0 &&
                    ((uintptr_t)stats & 7) == 0 && ((uintptr_t)ws & 15) == 0,
                ULTR_EINVAL, "%s: gamma, d_gamma, d_beta, stats or ws not aligned", who);
-  ULTR_REQUIRE(!rows_overlap(dx, lddx, x, ldx, M, N, x_dtype) && !rows_overlap(dx, lddx, dy, lddy, M, N, x_dtype), ULTR_EINVAL,
-               "%s: dx overlaps x or dy", who);
-  auto share = [&](const void* a, const void* b) {  // two weight vectors that overlap
-    const uintptr_t bytes = (uintptr_t)N * dtype_bytes(w_dtype), pa = (uintptr_t)a, pb = (uintptr_t)b;
-    return a && b && pa < pb + bytes && pb < pa + bytes;
-  };
-  ULTR_REQUIRE(!share(d_gamma, d_beta) && !share(gamma, d_gamma) && !share(gamma, d_beta), ULTR_EINVAL,
-               "%s: d_gamma overlaps d_beta, or one of them gamma", who);
   const bool dw = d_gamma || d_beta;
-  ULTR_REQUIRE((!dw && N <= kGradWidth) || ws || ultr_layer_norm_workspace_bytes(M, N) == 0, ULTR_EINVAL,
-               "%s: workspace required", who);
+  const long long ws_bytes = !dw && N <= kGradWidth ? 0 : ultr_layer_norm_workspace_bytes(M, N);
+  ULTR_REQUIRE(ws || ws_bytes == 0, ULTR_EINVAL, "%s: workspace required", who);
+  {
+    const long long w = (long long)N * dtype_bytes(w_dtype);
+    const Extent in[] = {matrix(x, ldx, M, N, x_dtype), matrix(dy, lddy, M, N, x_dtype), vector(stats, M * 8), vector(gamma, w)};
+    const Extent out[] = {matrix(dx, lddx, M, N, x_dtype), vector(d_gamma, w), vector(d_beta, w), vector(ws, ws_bytes)};
+    static const char* const in_name[] = {"x", "dy", "stats", "gamma"};
+    static const char* const out_name[] = {"dx", "d_gamma", "d_beta", "ws"};
+    for (int o = 0; o < 4; ++o) {
+      for (int i = 0; i < 4; ++i)
+        ULTR_REQUIRE(!touch(out[o], in[i]), ULTR_EINVAL, "%s: %s overlaps %s", who, out_name[o], in_name[i]);
+      for (int i = 0; i < o; ++i)
+        ULTR_REQUIRE(!touch(out[o], out[i]), ULTR_EINVAL, "%s: %s overlaps %s", who, out_name[o], out_name[i]);
+    }
+  }
   hipStream_t s = as_stream(stream);
   const float inv_n = 1.f / (float)N;
   return with_types(x_dtype, w_dtype, [&](auto* t, auto* w) {

@@ -83,7 +83,8 @@ def _stats(stats, shape, device):
 
 def layer_norm(x, gamma=None, beta=None, eps=LN_EPS, out=None, stats=None):
     """-> (out, stats): out = (x - mean) * rstd * gamma + beta over the last axis, stats[..., 0:2] = (mean, rstd) in float32
-    (the layout of ``feature_row_stats``).  ``out`` may be x itself; ``out`` / ``stats`` are allocated when not given."""
+    (the layout of ``feature_row_stats``).  ``out`` may be x itself or other columns of the table x is a slice of; no other
+    argument may share memory with ``out`` or ``stats``, which are allocated when not given."""
     dtype, code, device, shape = _input(x)
     m, ldx = _rows(x, shape, 'x')
     n = shape[-1]
@@ -124,7 +125,8 @@ def layer_norm_backward(d_out, x, stats, gamma=None, d_x=None, d_gamma=None, d_b
     """-> (d_x, d_gamma, d_beta) for ``layer_norm(x, gamma, ...)`` that returned ``stats``.
 
     ``need``: which of the three are wanted; the others come back as None.  Gradients are written, not added to;
-    d_gamma / d_beta have gamma's type (float32 without gamma) unless given.  d_x must not share memory with d_out or x."""
+    d_gamma / d_beta have gamma's type (float32 without gamma) unless given.  What is written (the workspace
+    too) must not share memory with another argument; d_x may be other columns of the table that x or d_out is a slice of."""
     dtype, code, device, shape = _input(x)
     m, ldx = _rows(x, shape, 'x')
     n = shape[-1]
