@@ -188,14 +188,16 @@ template <bool STREAM>
 __global__ void __launch_bounds__(kTThreads) tensors_sumsq_kernel(ListView l, const float* denom, float scale_const, float l2) {
   __shared__ double red[kTThreads / 64];
   const float sc = scale_of(denom, scale_const);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *l.scale = sc;
   double acc = 0.0;
   // whole turns of the grid, so that a chunk belongs to the same workgroup in both passes
   const long long past = STREAM ? max(l.n_chunks - kKeepChunks, 0ll) / gridDim.x * gridDim.x : 0;
   if (STREAM) for_chunks(l.chunks, past, false, [&](const ChunkRec& r) { add_squares<true>(r, sc, l2, acc); });
   for_chunks(l.chunks + past, l.n_chunks - past, false, [&](const ChunkRec& r) { add_squares<false>(r, sc, l2, acc); });
   acc = block_sum_f64(acc, red);
-  if (threadIdx.x == 0) l.partials[blockIdx.x] = acc;
+  if (threadIdx.x == 0) {
+    l.partials[blockIdx.x] = acc;
+    if (blockIdx.x == 0) *l.scale = sc;
+  }
 }
 
 __device__ __forceinline__ double partials_sum(const double* partials, int n, double* red) {
