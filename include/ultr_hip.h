@@ -581,6 +581,9 @@ typedef struct UltrTensorPlan {
   long long n_chunks; /* the list cut into chunks, none of which spans two tensors                      */
   int n_tensors;
   int has;            /* bits of what EVERY non-empty tensor has: 1 out, 2 param, 4 accum               */
+  long long keep_from;    /* the chunks from here on hold the last 256 MB of the gradients              */
+  long long clip_bytes;   /* what the second pass of a clip moves                                       */
+  long long update_bytes; /* and of an update                                                           */
 } UltrTensorPlan;
 
 /* Device bytes the table of this list takes (> 0 even for an empty list); -1 on a bad list. */

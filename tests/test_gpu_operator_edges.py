@@ -264,3 +264,51 @@ def test_python_calls_that_share_memory():
                  lambda: layer_norm_backward(dy, x, stats, d_beta=stats.view(-1)[:8])):
         with pytest.raises(_lib.UltrError, match='overlaps'):
             call()
+
+
+def test_what_a_list_moves_is_counted_in_bytes():
+    from ultra_amd.learning_algorithm import GradientTensors
+    tiny = GradientTensors(list(torch.randn(200000, device='cuda').split(10)))
+    out, norm = tiny.clip(1.0)
+    p = tiny._plan.contents
+    assert (p.n_chunks, p.clip_bytes, p.update_bytes, p.keep_from) == (20000, 200000 * 8, 200000 * 12, 0)
+    want = ref_norm(tiny.grads)
+    assert abs(float(norm) - want) <= 4 * U * want
+    within(torch.cat(out), torch.cat(tiny.grads).double() / want, 4 * U * torch.cat(tiny.grads).abs().double() + half_step(F32, norm), 'out')
+    mixed = [torch.zeros(n, dtype=t, device='cuda') for n, t in ((4097, BF16), (1000, F32), (0, F16))]
+    plan = GradientTensors(mixed, params=[torch.zeros(m.shape, device='cuda') for m in mixed],
+                           accums=[torch.zeros(m.shape, device='cuda') for m in mixed],
+                           copies=[torch.zeros(4097, dtype=F16, device='cuda'), None, None])._plan.contents
+    assert (plan.n_chunks, plan.clip_bytes, plan.update_bytes, plan.keep_from) == (3, 4097 * 4 + 1000 * 8, 4097 * 20 + 1000 * 20, 0)
+
+
+@pytest.mark.parametrize('sizes,dtypes,chunks', [
+    ([150000001, 4097], (BF16,), 36622 + 2 - 32768 + 1), ([70000003, 9], (F32,), 17090 + 1 - 16384 + 1),
+    ([40000001, 70000000, 8193], (F32, BF16), None), ([5, 300000001], (F16,), 1 + 73243 - 32768)])
+def test_first_passes_that_change_over(sizes, dtypes, chunks):
+    """Gradients beyond 256 MB: the first ones are read past the caches, the last 256 MB are not.  Every chunk is counted once,
+    with the parameters' part of the norm too."""
+    from ultra_amd.learning_algorithm import GradientTensors
+    grads, params = tensors(sizes, dtypes, 1, aligned=False), tensors(sizes, (F32,), 2, aligned=False)
+    plan = GradientTensors(grads, out=[torch.empty_like(g) for g in grads], params=params)
+    p = plan._plan.contents
+    assert 0 < p.keep_from < p.n_chunks
+    if chunks is not None:
+        assert abs(p.keep_from - chunks) <= 1
+    kept = sum(g.numel() * g.element_size() for g in grads)
+    assert kept > 256 << 20 and p.clip_bytes == 2 * kept
+    want = ref_norm(grads)
+    out, norm = plan.clip(1.0)
+    assert abs(float(norm) - want) <= 4 * U * want and abs(float(plan.global_norm()) - want) <= 4 * U * want
+    for o, g in zip(out, grads):
+        w = g.double() / want
+        within(o, w, 4 * U * w.abs() + half_step(g.dtype, w), 'out')
+        del w
+    with_l2 = sum(float((g.double() + 0.01 * q.double()).square().sum()) for g, q in zip(grads, params)) ** 0.5
+    before = [q.clone() for q in params]
+    got = plan.clip_adagrad(1.0, 0.5, l2=0.01, grad_strategy='sgd')
+    assert abs(float(got) - with_l2) <= 8 * U * with_l2
+    for q, b, g in zip(params, before, grads):
+        step = (g.double() + 0.01 * b.double()) * (0.5 / with_l2)
+        tol = 9 * U * (g.double().abs() + 0.01 * b.double().abs()) * (0.5 / with_l2) + U * 2 * b.abs()
+        within(q, b.double() - step, tol, 'param')

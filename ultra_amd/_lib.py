@@ -67,6 +67,9 @@ class UltrTensorPlan(ctypes.Structure):
         ('n_chunks', ctypes.c_longlong),
         ('n_tensors', ctypes.c_int),
         ('has', ctypes.c_int),
+        ('keep_from', ctypes.c_longlong),
+        ('clip_bytes', ctypes.c_longlong),
+        ('update_bytes', ctypes.c_longlong),
     ]
 
 

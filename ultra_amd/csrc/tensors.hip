@@ -15,12 +15,16 @@ namespace ultr {
 constexpr int kTThreads = 256;
 constexpr int kChunk = 4096;       // elements of one tensor that one workgroup takes at a time
 constexpr int kTMaxBlocks = 1536;  // workgroups of a pass, and partial sums of a norm
-// Lists of more chunks than this (64 M elements: their second pass moves 256 MB or more) do not fit the 256 MB last-level
-// cache: what will not be read again goes past the caches (NT), so that the last gradients of the first pass are still there
-// when the second one begins with them.  Clip of 553 M bf16: 542 us, 625 without; update of 151 M: 564 us, 666 without.
-// Lists that fit lose by it (1000 ragged tensors, 22 MB: 19.3 us against 15.8) and leave their outputs in the caches.
-constexpr long long kStreamChunks = 16384;
-constexpr long long kKeepChunks = 2 * kStreamChunks;  // the end of the list that the first pass leaves in the caches
+// The last-level cache.  A second pass that moves more than this sends its data past the caches (NT): nothing of it would be there
+// when something reads it again.  One that moves less leaves its outputs there, and its inputs may lie there already.  One
+// list again and again, NT against plain: clip of fp32 224 MB 54.8 us and 53.3, 256 MB 61.9 and 61.8, 288 MB 69.8 and
+// 72.6, 384 MB 92 and 101; of bf16 320 MB 75.6 and 80.6; update 200 MB 43.0 and 43.9, 320 MB 65.3 and 66.2, 480 MB 95 and
+// 100.  (Three lists in turn, whose data the caches do not hold, gain from 128 MB on: 32.4 us and 38.0.)  60000 tensors of ten
+// elements, 5 MB: 88 us and 78.
+// A first pass over more gradients than this does the same, but for the last gradients of that size, with which the second pass
+// begins (clip of 553 M bf16: 542 us, 625 without both; update of 151 M: 564 us, 666 without both; the last 128 MB or 512
+// MB instead of 256 lose 0 to 4 %).
+constexpr long long kCacheBytes = 256ll << 20;
 
 struct ChunkRec {  // what one chunk needs: its tensor's pointers, moved to its first element
   const void* grad;
@@ -44,9 +48,10 @@ struct ListView {
   float* scale;  // what the first pass made of denom: the second one may be overwriting that memory
   const ChunkRec* chunks;
   long long n_chunks;
+  long long keep_from;  // the chunks from here on hold the last kCacheBytes of the gradients
 };
 
-constexpr int kFillTensors = 48;  // tensors per fill launch: they travel as kernel arguments (3.5 KB)
+constexpr int kFillTensors = 48;  // tensors per fill launch: they travel as kernel arguments (3 KB)
 struct FillArgs {
   UltrTensor t[kFillTensors];
   long long first_chunk[kFillTensors];
@@ -190,7 +195,7 @@ __global__ void __launch_bounds__(kTThreads) tensors_sumsq_kernel(ListView l, co
   const float sc = scale_of(denom, scale_const);
   double acc = 0.0;
   // whole turns of the grid, so that a chunk belongs to the same workgroup in both passes
-  const long long past = STREAM ? max(l.n_chunks - kKeepChunks, 0ll) / gridDim.x * gridDim.x : 0;
+  const long long past = STREAM ? l.keep_from / gridDim.x * gridDim.x : 0;
   if (STREAM) for_chunks(l.chunks, past, false, [&](const ChunkRec& r) { add_squares<true>(r, sc, l2, acc); });
   for_chunks(l.chunks + past, l.n_chunks - past, false, [&](const ChunkRec& r) { add_squares<false>(r, sc, l2, acc); });
   acc = block_sum_f64(acc, red);
@@ -368,24 +373,36 @@ static int check_overlap(const char* who, const UltrTensor* t, int n) {
   return ULTR_OK;
 }
 
+// The first chunk of those, counted from the end of the list, that hold kCacheBytes of gradients.
+static long long keep_from(const UltrTensor* t, int n, long long n_chunks) {
+  long long left = kCacheBytes, chunk = n_chunks;
+  for (int i = n - 1; i >= 0; --i) {
+    const long long each = (long long)kChunk * dtype_bytes(t[i].grad_dtype), count = cdiv(t[i].n, kChunk);
+    if (count * each > left) return chunk - left / each;
+    left -= t[i].n * dtype_bytes(t[i].grad_dtype);
+    chunk -= count;
+  }
+  return 0;
+}
+
 static int check_plan(const char* who, const UltrTensorPlan* p, int need, float clip_norm) {
   ULTR_REQUIRE(clip_norm == clip_norm, ULTR_EINVAL, "%s: clip_norm is not a number", who);
-  ULTR_REQUIRE(p && p->table && p->n_chunks >= 0 && p->n_tensors >= 0, ULTR_EINVAL, "%s: bad plan", who);
+  ULTR_REQUIRE(p && p->table && p->n_chunks >= 0 && p->n_tensors >= 0 && p->keep_from >= 0 && p->keep_from <= p->n_chunks, ULTR_EINVAL,
+               "%s: bad plan", who);
   ULTR_REQUIRE((p->has & need) == need, ULTR_EINVAL, "%s: the list lacks%s%s%s", who, (need & ~p->has & 1) ? " out" : "",
                (need & ~p->has & 2) ? " param" : "", (need & ~p->has & 4) ? " accum" : "");
   return ULTR_OK;
 }
 static ListView view_of(const UltrTensorPlan* p) {
   char* b = static_cast<char*>(p->table);
-  return ListView{reinterpret_cast<double*>(b), reinterpret_cast<float*>(b + kPartialBytes), reinterpret_cast<const ChunkRec*>(b + kHeadBytes), p->n_chunks};
+  return ListView{reinterpret_cast<double*>(b), reinterpret_cast<float*>(b + kPartialBytes), reinterpret_cast<const ChunkRec*>(b + kHeadBytes), p->n_chunks, p->keep_from};
 }
-static bool streams(const ListView& l) { return l.n_chunks > kStreamChunks; }
 static int pass_blocks(long long n_chunks) { return (int)std::min<long long>(n_chunks, kTMaxBlocks); }
 
 static int launch_sumsq_blocks(const ListView& l, int nb, const float* denom, float scale_const, float l2, hipStream_t s) {
   {
     ProfScope prof_("tensors_sumsq_kernel", s);
-    hipLaunchKernelGGL(streams(l) ? tensors_sumsq_kernel<true> : tensors_sumsq_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, denom, scale_const, l2);
+    hipLaunchKernelGGL(l.keep_from > 0 ? tensors_sumsq_kernel<true> : tensors_sumsq_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, denom, scale_const, l2);
   }
   return check_launch("tensors_sumsq_kernel");
 }
@@ -398,7 +415,7 @@ static int launch_sumsq(const ListView& l, const float* denom, float scale_const
 }
 // The scale alone, for an update that forms no norm: the first pass over no chunk at all.
 static int launch_scale(ListView l, const float* denom, float scale_const, hipStream_t s) {
-  l.n_chunks = 0;
+  l.n_chunks = l.keep_from = 0;
   return launch_sumsq_blocks(l, 1, denom, scale_const, 0.f, s);
 }
 static int launch_norm(const ListView& l, int n_partials, float* out_norm, hipStream_t s) {
@@ -460,7 +477,13 @@ extern "C" int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, voi
     rc = check_launch("tensors_fill_kernel");
     if (rc) return rc;
   }
-  *plan_h = UltrTensorPlan{table, chunks, n_tensors, has};
+  *plan_h = UltrTensorPlan{table, chunks, n_tensors, has, keep_from(tensors_h, n_tensors, chunks), 0, 0};
+  for (int i = 0; i < n_tensors; ++i) {
+    const UltrTensor& t = tensors_h[i];
+    const long long g = dtype_bytes(t.grad_dtype);
+    plan_h->clip_bytes += t.n * 2 * g;
+    plan_h->update_bytes += t.n * (g + 8 + (t.accum ? 8 : 0) + (t.copy ? dtype_bytes(t.copy_dtype) : 0));
+  }
   return ULTR_OK;
 }
 
@@ -485,7 +508,7 @@ extern "C" int ultr_clip_by_global_norm(const UltrTensorPlan* plan_h, const floa
   if (nb == 0) return out_norm ? launch_norm(l, 0, out_norm, s) : ULTR_OK;
   {
     ProfScope prof_("tensors_clip_kernel", s);
-    hipLaunchKernelGGL(streams(l) ? tensors_clip_kernel<true> : tensors_clip_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, nb, clip_norm, out_norm);
+    hipLaunchKernelGGL(plan_h->clip_bytes > kCacheBytes ? tensors_clip_kernel<true> : tensors_clip_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, nb, clip_norm, out_norm);
   }
   return check_launch("tensors_clip_kernel");
 }
@@ -511,7 +534,7 @@ extern "C" int ultr_clip_adagrad_tensors(const UltrTensorPlan* plan_h, const flo
   }
   {
     ProfScope prof_("tensors_update_kernel", s);
-    hipLaunchKernelGGL(streams(l) ? tensors_update_kernel<true> : tensors_update_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, np, np > 0 || denom, scale_const, l2, clip_norm, lr,
+    hipLaunchKernelGGL(plan_h->update_bytes > kCacheBytes ? tensors_update_kernel<true> : tensors_update_kernel<false>, dim3(nb), dim3(kTThreads), 0, s, l, np, np > 0 || denom, scale_const, l2, clip_norm, lr,
                        strategy, out_norm);
   }
   return check_launch("tensors_update_kernel");
