@@ -312,3 +312,22 @@ def test_first_passes_that_change_over(sizes, dtypes, chunks):
         step = (g.double() + 0.01 * b.double()) * (0.5 / with_l2)
         tol = 9 * U * (g.double().abs() + 0.01 * b.double().abs()) * (0.5 / with_l2) + U * 2 * b.abs()
         within(q, b.double() - step, tol, 'param')
+
+
+def test_a_list_whose_outputs_could_not_be_laid_out(monkeypatch):
+    from ultra_amd import _lib
+    from ultra_amd.learning_algorithm import GradientTensors
+    grads = tensors([5000, 3], (F32,), 1)
+    want = ref_norm(grads)
+    plan = GradientTensors(grads)
+
+    def fails(rc, what):
+        raise _lib.UltrError('no')
+    with monkeypatch.context() as m:
+        m.setattr(_lib, 'check', fails)
+        with pytest.raises(_lib.UltrError):
+            plan.clip(1.0)
+    assert plan.out is None and len(plan._tables) == 1
+    assert abs(float(plan.global_norm()) - want) <= 4 * U * want
+    out, _ = plan.clip(want / 2)
+    within(out[0], grads[0].double() / 2, 5 * U * grads[0].double().abs(), 'out')

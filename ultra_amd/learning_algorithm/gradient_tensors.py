@@ -91,14 +91,14 @@ class GradientTensors(object):
         if nbytes < 0:
             raise _lib.UltrError(lib.ultr_last_error().decode())
         table = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-        self._tables.append(table)  # an earlier one stays: a captured graph may read it
-        self._streams = set()  # that have used it
         plan = _lib.UltrTensorPlan()
         _lib.check(lib.ultr_tensors_plan(ptr, n, _lib.ptr(table), nbytes, plan, _lib.current_stream()), 'ultr_tensors_plan')
         self._tell_scorers(rec)
         # whichever stream uses the plan later finds it written
         torch.cuda.current_stream().synchronize()
         self._plan = ctypes.pointer(plan)
+        self._tables.append(table)  # an earlier one stays: a captured graph may read it
+        self._streams = set()  # that have used it
 
     @staticmethod
     def _tell_scorers(rec):
@@ -144,7 +144,11 @@ class GradientTensors(object):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('clip: give ``out`` to the constructor before capturing')
             self.out = [torch.empty_like(g) for g in self.grads]
-            self._build()
+            try:
+                self._build()
+            except Exception:
+                self.out = None
+                raise
         rc = _lib._lib.ultr_clip_by_global_norm(self._plan, self._denom(denom), scale, clip_norm, self._norm_ptr, self._stream())
         if rc:
             _lib.check(rc, 'ultr_clip_by_global_norm')
