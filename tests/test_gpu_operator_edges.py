@@ -331,3 +331,15 @@ def test_a_list_whose_outputs_could_not_be_laid_out(monkeypatch):
     assert abs(float(plan.global_norm()) - want) <= 4 * U * want
     out, _ = plan.clip(want / 2)
     within(out[0], grads[0].double() / 2, 5 * U * grads[0].double().abs(), 'out')
+
+
+def test_a_first_clip_on_another_device(monkeypatch):
+    """The outputs are laid out by kernels, on the list's device only."""
+    from ultra_amd.learning_algorithm import GradientTensors, gradient_tensors
+    plan = GradientTensors(tensors([5000, 3], (F32,), 1))
+    with monkeypatch.context() as m:
+        m.setattr(gradient_tensors, '_current_device', lambda: plan._index + 1)
+        with pytest.raises(ValueError, match='current device'):
+            plan.clip(1.0)
+    assert plan.out is None and len(plan._tables) == 1
+    plan.clip(1.0)

@@ -143,6 +143,7 @@ class GradientTensors(object):
         if self.out is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError('clip: give ``out`` to the constructor before capturing')
+            self._stream()  # the list is laid out on its own device
             self.out = [torch.empty_like(g) for g in self.grads]
             try:
                 self._build()
