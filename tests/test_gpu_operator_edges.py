@@ -343,3 +343,70 @@ def test_a_first_clip_on_another_device(monkeypatch):
             plan.clip(1.0)
     assert plan.out is None and len(plan._tables) == 1
     plan.clip(1.0)
+
+
+# ---- forms that other tests pass by ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize('m,n', [(2048, 300), (2049, 700), (3001, 1030), (2051, 2048), (2048, 4096), (2049, 4097), (2050, 5003), (2049, 8200),
+                                 (2051, 16384), (2049, 16385), (2100, 1052)])
+def test_forward_of_two_rows_a_thread_group(m, n):
+    """From 2048 rows on a thread group forms two rows: whole waves, several waves, odd last rows, odd widths, in a table, in place."""
+    from tests.test_gpu_layer_norm import TYPES, ref_forward, rows, weights
+    from ultra_amd.ranking_model import layer_norm
+    for k, (t, w) in enumerate(TYPES):
+        x, _ = rows(m, n, t, k, gap=5 * (k % 2), shift=k % 3, scale=1.5, offset=0.7)
+        gamma, beta = weights(n, w, k + 10)
+        ry, rs, ty, ts = ref_forward(x, gamma, beta)
+        y, buf = rows(m, n, t, 99, gap=3, shift=1)
+        before = buf.clone()
+        _, stats = layer_norm(x, gamma, beta, out=y)
+        within(stats, rs, ts, 'stats %s' % t)
+        within(y, ry, ty, 'y %s %s' % (t, w))
+        keep = torch.ones_like(buf, dtype=torch.bool)
+        keep[1:].view(m, n + 3)[:, :n] = False
+        assert torch.equal(buf[keep], before[keep])
+        layer_norm(x, gamma, beta, out=x)
+        assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize('m,n', [(1025, 16392), (1100, 16385), (1030, 20000), (2049, 17001), (1025, 32768), (1026, 40007), (1025, 65536)])
+def test_backward_of_many_wide_rows(m, n):
+    """16-bit rows beyond 16384 and fp32 rows beyond 8192, more than 1024 of them: column tiles times row slices."""
+    from tests.test_gpu_layer_norm import TYPES, ref_backward, ref_forward, rows, weights
+    from ultra_amd.ranking_model import layer_norm, layer_norm_backward
+    for k, (t, w) in enumerate(TYPES):
+        x, _ = rows(m, n, t, k, gap=3 * (k % 2), shift=k % 2, scale=1.5, offset=0.4)
+        dy, _ = rows(m, n, t, k + 50)
+        gamma, _ = weights(n, w, k)
+        _, stats = layer_norm(x)
+        _, rs, _, ts = ref_forward(x, None, None)
+        within(stats, rs, ts, 'stats')
+        d_x, buf = rows(m, n, t, 99, gap=5, shift=1)
+        before = buf.clone()
+        dx, dg, db = layer_norm_backward(dy, x, stats, gamma, d_x=d_x)
+        rx, rg, rb, tx, tg, tb = ref_backward(dy, x, stats, gamma)
+        within(dx, rx, tx, 'dx %s' % t)
+        within(dg, rg, tg + half_step(w, rg), 'd_gamma %s' % w)
+        within(db, rb, tb + half_step(w, rb), 'd_beta %s' % w)
+        keep = torch.ones_like(buf, dtype=torch.bool)
+        keep[1:].view(m, n + 5)[:, :n] = False
+        assert torch.equal(buf[keep], before[keep])
+        del rx, tx, keep, before
+        again = layer_norm_backward(dy, x, stats, gamma)
+        assert all(torch.equal(p, q) for p, q in zip((dx, dg, db), again))
+        only = layer_norm_backward(dy, x, stats, gamma, need=(False, True, True))
+        assert torch.equal(only[1], dg) and torch.equal(only[2], db)
+        only = layer_norm_backward(dy, x, stats, gamma, need=(True, False, False))
+        assert torch.equal(only[0], dx)
+
+
+@pytest.mark.parametrize('m,n', [(16, 136), (700, 512), (3000, 700), (1030, 8200), (600, 9001)])
+def test_statistics_that_a_gradient_takes(m, n):
+    """The gradient's tests take the forward pass's statistics as given; here they are checked at such sizes."""
+    from tests.test_gpu_layer_norm import TYPES, ref_forward, rows
+    from ultra_amd.ranking_model import layer_norm
+    for k, (t, _) in enumerate(TYPES):
+        x, _ = rows(m, n, t, k, scale=1.5, offset=0.4)
+        y, stats = layer_norm(x)
+        ry, rs, ty, ts = ref_forward(x, None, None)
+        within(stats, rs, ts, 'stats')
+        within(y, ry, ty, 'y')
