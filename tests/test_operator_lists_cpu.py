@@ -49,3 +49,13 @@ def test_a_list_after_the_capture_is_refused():
     written(param=(first.params.data_ptr() + 4, 0))  # before the capture: nothing that a graph could rely on
     first._wt_captured = True
     written(param=(first.params.data_ptr() + 4, 0))
+
+
+def test_a_copied_scorer_is_known_too():
+    import copy
+    m = scorer()
+    twin, alias = copy.deepcopy(m), copy.copy(m)
+    written(param=(twin.params.data_ptr(), 0))
+    assert not twin._wt_kept and m._wt_kept and alias._wt_kept
+    written(param=(m.params.data_ptr(), 0))
+    assert not m._wt_kept and not alias._wt_kept

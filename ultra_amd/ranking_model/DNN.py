@@ -32,6 +32,9 @@ def _round_up(x, m):
 
 
 class DNN(BaseRankingModel):
+    _wt_kept = True       # what the scorer's own last update left of the fused step's weight copies may be used
+    _wt_captured = False  # a captured fused step uses it
+
     def __init__(self, hparams_str):
         self.hparams = hp.HParams(
             hidden_layer_sizes=[512, 256, 128],  # neurons per hidden layer
@@ -50,8 +53,12 @@ class DNN(BaseRankingModel):
         self._last = None
         self._last_fused = None
         self._wt_state = None
-        self._wt_kept = True       # what the scorer's own last update left of the fused step's weight copies may be used
-        self._wt_captured = False  # a captured fused step uses it
+
+    def __setstate__(self, state):  # a copy's parameters can be listed too
+        self.__dict__.update(state)
+        if self.params is not None:
+            with _scorers_lock:
+                _scorers.add(self)
 
     # ---- variables -------------------------------------------------------------------------
     def layer_shapes(self, feature_size):
