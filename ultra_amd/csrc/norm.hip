@@ -21,9 +21,9 @@ static void first_shape(int N, F&& fn, S... shapes) {
   (void)((N <= S::TPR * S::C * S::V ? (fn(shapes), true) : false) || ...);
 }
 // Forward: two 16-byte pieces a thread until a workgroup is full, then more (fp32: one or four lose 2 to 10 %).  16-bit rows
-// that fill twice the threads with one piece each take those (16384 rows of 4096 bf16, fp32 weights: 50 us, 52 with two
-// pieces); where many threads would be idle they do not (16969 rows of 1052 fp16: 21 us, 17 with two pieces; 1592 of 2048
-// threads' worth: 14.9 and 13.2).  Rows shorter than one piece: element by element.
+// that fill twice the threads with one piece each take those (16384 rows of 4096 bf16, fp32 weights: 49.4 us, 51.6 with two
+// pieces); where many threads would be idle they do not (16969 rows of 1052 fp16: 21.7 us, 18.4 with two pieces; 1592 of 2048
+// threads' worth: 15.2 and 13.6).  Rows shorter than one piece: element by element.
 template <typename T, typename F>
 static void forward_shape(int N, F&& fn) {
   if constexpr (sizeof(T) == 4) {
@@ -45,7 +45,8 @@ static void forward_shape(int N, F&& fn) {
   }
 }
 // Backward: 16 elements a thread, up to the 512 threads of a workgroup; 16-bit rows then 32 (4096 rows of 16384 bf16: 87 us,
-// 129 in column tiles; 1500 rows: 44 and 54; fp32 spills), and rows that are only held for a moment (FEW) what fits.
+// 129 in column tiles; 1500 rows: 44 and 54), though that spills 5 to 7 of 256 registers; fp32 rows would spill what they
+// prefetch, and rows that are only held for a moment (FEW) what fits.
 constexpr int kGradWidth = 16 * kGradThreads;
 constexpr int kHeldWidth16 = 2 * kGradWidth;
 constexpr int kFewWidth32 = 32768;  // 16-bit types: every width
@@ -212,8 +213,11 @@ extern "C" int ultr_layer_norm_forward(const void* x, long long ldx, const void*
                              (T*)y + m * ldy, ldy, stats ? stats + 2 * m : nullptr);
         }
       };
-      // two rows a thread group once there are rows enough to fill the chip that way (512 rows of 4096 bf16: 4.5 us with
-      // one, 4.8 with two; 4096 rows: 18.1 and 16.4), and registers for both
+      // two rows a thread group once there are rows enough to fill the chip that way, and registers for both: it is for
+      // matrices beyond the caches with weights as wide (one row against two: 16384 x 4096 bf16 56.3 us and 49, with fp32
+      // weights 60.8 and 50.4; 30010 x 5003 fp16 160 and 124; 3001 x 5003 15.9 and 15.2; 2048 x 4096 fp32 13.0 and
+      // 12.1).  Those that the caches hold and narrow rows are within 10 % either way (4096 x 4096 bf16 14.6 and
+      // 15.5; 40960 x 512 fp32 30.6 and 31.2; 16969 x 1052 fp16 18.0 and 19.0; 40960 x 700 fp32 42.8 and 42.0).
       constexpr bool pair = S::C * S::V * sizeof(T) <= 64;
       auto rows = [&](auto tail) {
         if constexpr (pair) {
@@ -323,10 +327,12 @@ extern "C" int ultr_layer_norm_backward(const void* dy, long long lddy, const vo
           hipLaunchKernelGGL((layer_norm_row_sums_kernel<T, W, V, TAIL, NT>), dim3((unsigned)std::min<long long>(M, 2048)), dim3(NT),
                              0, s, (const T*)dy, lddy, (const T*)x, ldx, stats, (const W*)gamma, M, N, inv_n, sums);
         };
-        // many rows: small workgroups, more rows at a time (4096 rows of 16384 bf16: 50 us, 60 with 1024 threads); the few
-        // that come here, fp32 beyond the width of the few-rows pass, take all the threads a workgroup can have
+        // 16-bit rows that come here: small workgroups, more rows at a time (whole call, 256 threads against 1024: 3000 x
+        // 20001 bf16 158 us and 169, 8192 x 20000 fp16 324 and 334, 2048 x 32768 bf16 131 and 134, though 1100 x 65536
+        // 163 and 151).  fp32 rows that give 1024 threads three pieces each: all of them (4096 x 16384 283 us and 273,
+        // 2000 x 12345 110 and 104.5, 1100 x 32768 165 and 150, 8 x 65536 33.6 and 17.8; 1100 x 9000 41.8 and 42.7).
         if (dx) {
-          if (sizeof(T) == 2 || M > 512) row_sums_of(std::integral_constant<int, 256>{});
+          if (sizeof(T) == 2 || N < 3 * 1024 * V) row_sums_of(std::integral_constant<int, 256>{});
           else row_sums_of(std::integral_constant<int, sizeof(T) == 2 ? 256 : 1024>{});
         }
         ProfScope prof_("layer_norm_wide_grad_kernel", s);
