@@ -87,9 +87,11 @@ struct Pieces {
 
 // Forward.  HBM-bound: one read and one write of the matrix.  TPR threads hold R whole rows in registers, so the mean, the
 // variance about it and the output need one pass over memory.  R = 2: the weights, which come out of the caches once per
-// row otherwise, serve two rows (fp16 rows of 5003 with fp32 weights, 30010 of them: 117 us against 158).  Narrow rows
-// ask for their weights along with the row (136 fp32: 5.0 TB/s against 4.3); in a workgroup of several waves the other
-// workgroups cover that latency and the registers are worth more (8192 fp32, R = 2: 5.6 TB/s against 4.7).
+// row otherwise, serve two rows (fp16 rows of 5003 with fp32 weights, 30010 of them: 124 us against 160; they still move as
+// many bytes of weights out of the caches as of the matrix).  Narrow rows ask for their weights along with the row (40960 x
+// 136 fp32: 8.8 us against 9.9); in a workgroup of several waves the other workgroups cover that latency and the registers
+// are worth more (two rows at a time, early against late: the 30010 rows in the kernel alone 126 us and 113, 16384 x 4096 bf16
+// 48.6 and 47.4; fp32 is within 2.5 % either way, 8192 x 4096 47.5 and 48.6, 4096 x 8192 49.9 and 50.7).
 //
 // The mean is mean[r] + low[r]: an error of a fraction of the row's OFFSET would be the whole variance of a row that hardly
 // varies (a constant row of 1e6, 5003 entries, came out as 0.9).  That costs 0 to 2 % over one fp32 sum, up to 5 % in
@@ -334,6 +336,10 @@ __global__ void __launch_bounds__(kGradThreads)
 // mostly out of a cache the second time; the pass above writes and re-reads partial rows instead, and takes a second launch.
 // 100 rows of 4096 bf16: 5.5 us, 9.0 the other way; 512 rows: 9.7 and 11.8; beyond, narrow rows lose by it (1000 rows of 136
 // fp32: 12.4 and 6.5) and rows of more than 8192 gain up to about 1024 (777 rows of 12345 bf16: 22 us, 29 in column tiles).
+// What bounds it there is not the memory: the workgroups that form dx, alone, take 20.2 us of the 777 x 12345 case, those that
+// sum columns 20.9 alone, and their second reading mostly comes from the last-level cache.  A workgroup loads a row, sums and
+// stores with nothing on its way meanwhile, and two of them fit a CU (97 to 101 registers): 512 rows at a time, so that 777 rows
+// are two turns (the dx half alone: 512 rows 12.5 us, 777 rows 20.2, 1000 rows 22.1).
 //
 // Columns: the threads of a workgroup as `rt` row threads times NT / rt threads of V columns each (8 at least: 128 bytes).
 template <typename T, typename W, int V, bool TAIL, int NT>
@@ -454,7 +460,9 @@ __global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR)
 // Backward, rows wider than that: the two sums of every row first, then a pass in which a workgroup owns a column tile and
 // a slice of the rows.  Reads the matrices twice; nothing but the two sums crosses threads.  The slice is the fastest index
 // of that pass's grid and a multiple of 8, so that (workgroups go to the 8 XCDs in turn) an XCD meets the rows whose sums
-// it formed, the last ones first: its L2 may still hold them (512 rows of 65536 bf16 in this pass: 77 us, other orders 81).
+// it formed, the last ones first: its L2 may still hold them (whole call; first ones first; one slice more, no multiple of 8:
+// 2048 x 32768 bf16 131 us, 136, 133; 4096 x 16384 fp32 283, 294, 290; 512 x 65536 fp32 138, 154, 138; 3000 x 20001
+// bf16 158, 166, but 144).
 template <typename T, typename W, int V, bool TAIL, int NT>
 __global__ void __launch_bounds__(NT)
     layer_norm_row_sums_kernel(const T* dy, long long lddy, const T* x, long long ldx, const float* stats, const W* gamma,
