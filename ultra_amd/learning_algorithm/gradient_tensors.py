@@ -103,13 +103,15 @@ class GradientTensors(object):
     @staticmethod
     def _tell_scorers(rec):
         """The scorers learn which memory the calls on this list write."""
-        size = np.array([4, 2, 2], dtype=np.uint64)  # bytes of a DTYPE_*
-        begin, end = [], []
-        for name, each in (('out', size[rec['grad_dtype']]), ('param', 4), ('accum', 4), ('copy', size[rec['copy_dtype']])):
-            there = (rec[name] != 0) & (rec['n'] > 0)
-            begin.append(rec[name][there])
-            end.append((rec[name] + rec['n'].astype(np.uint64) * np.asarray(each, dtype=np.uint64))[there])
-        parameters_written(np.concatenate(begin), np.concatenate(end))
+        def memory():
+            size = np.array([4, 2, 2], dtype=np.uint64)  # bytes of a DTYPE_*
+            begin, end = [], []
+            for name, each in (('out', size[rec['grad_dtype']]), ('param', 4), ('accum', 4), ('copy', size[rec['copy_dtype']])):
+                there = (rec[name] != 0) & (rec['n'] > 0)
+                begin.append(rec[name][there])
+                end.append((rec[name] + rec['n'].astype(np.uint64) * np.asarray(each, dtype=np.uint64))[there])
+            return np.concatenate(begin), np.concatenate(end)
+        parameters_written(memory)
 
     def _stream(self):
         if _current_device() != self._index:

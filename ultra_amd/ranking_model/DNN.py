@@ -287,12 +287,14 @@ class DNN(BaseRankingModel):
         return [scores[l].view(B, 1) for l in range(L)]
 
 
-def parameters_written(begin, end):
-    """Calls that go round a scorer's own update will write the device memory [begin[k], end[k]) (uint64 arrays) whenever they
-    run or a graph replays them, unseen by torch's version counters.  A scorer whose parameters lie in it makes its weight
+def parameters_written(memory):
+    """Calls that go round a scorer's own update will write the device memory [begin[k], end[k]) (uint64 arrays, what ``memory``
+    returns) whenever they run or a graph replays them, unseen by torch's version counters.  A scorer whose parameters lie in it makes its weight
     copies anew in every fused step from now on; one of which a graph already holds a step that does not is refused."""
     with _scorers_lock:
         scorers = list(_scorers)
+    if scorers:
+        begin, end = memory()
     for s in scorers:
         lo = s.params.data_ptr()
         if not ((begin < lo + 4 * s.params.numel()) & (end > lo)).any():
