@@ -605,7 +605,8 @@ int ultr_tensors_plan(const UltrTensor* tensors_h, int n_tensors, void* table, l
 int ultr_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float* out_norm, void* stream);
 
 /* out = f * scale * grad for every tensor, f = clip_norm / max(norm, clip_norm) with the norm above (also written to
- * out_norm if that is not NULL).  clip_norm <= 0: f = 1; NaN is refused.  A norm that is not finite makes f NaN, and so every output
+ * out_norm if that is not NULL).  clip_norm <= 0: f = 1; NaN is refused.  f is an fp32 value: below 2^-126 (a norm of more
+ * than 8e37 times clip_norm) it loses bits.  A norm that is not finite makes f NaN, and so every output
  * NaN (as the reference's clip does).  Needs `out` in every tensor. */
 int ultr_clip_by_global_norm(const UltrTensorPlan* plan_h, const float* denom, float scale_const, float clip_norm,
                              float* out_norm, void* stream);

@@ -100,7 +100,7 @@ struct Pieces {
 //   16 bit  an fp32 sum is exact for entries of similar size (up to a factor of 4 for 2048 of them with 11 bits or 8192 with 8),
 //           and where they are not their spread is large against its roundings; longer rows meet in 64 bits from wave to wave.  So
 //           low is what the sum's quotient has beyond fp32 and needs no second sum.
-// Sums run in units of 2^kSumShift, so that no row of finite entries overflows.
+// Sums run in units of 2^kSumShift, so that no sum of finite entries overflows.
 //
 // x - mean must mean the same everywhere: the product that makes the mean is not to be fused into it.
 __device__ __forceinline__ float rounded_product(float a, float b) {
